@@ -123,6 +123,14 @@ def _declare(L: C.CDLL) -> None:
     L.dk_moe_ep_workspace_bytes.restype = sz
     L.dk_moe_ep_workspace_bytes.argtypes = [i, i, i, i, i, i]
     L.dk_moe_ep_layer.argtypes = [C.POINTER(DkMoeEpArgs), C.POINTER(DkView), C.c_uint, i, vp]
+    f = C.c_float
+    L.dk_add_rms_norm.argtypes = [vp, vp, vp, i, i, i, i, f, vp, vp, vp, vp]
+    L.dk_add_rms_norm_mx.argtypes = [vp, vp, vp, i, i, i, i, f, vp, vp, vp, vp, vp]
+    L.dk_add_rms_norm_bwd_workspace_bytes.restype = sz
+    L.dk_add_rms_norm_bwd_workspace_bytes.argtypes = [i, i]
+    L.dk_add_rms_norm_bwd.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp, vp, vp, sz, vp]
+    L.dk_gated_ffn.argtypes = [vp, vp, vp, i, i, i, vp, vp, vp, vp]
+    L.dk_gated_ffn_bwd.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, vp, vp, vp, vp, vp]
     L.dk_peer_barrier.argtypes = [C.POINTER(DkView), vp]
     L.dk_peer_barrier_epoch.argtypes = [C.POINTER(DkView), C.c_uint, vp]
     L.dk_set_peer_wait_ms.argtypes = [i]
@@ -498,6 +506,106 @@ def moe_ffn_mxfp8(xq, x_atoms, w13q, w13_atoms, w2q, w2_atoms, offsets, stream=N
     """gate/up + SiLU*mul + requantise, then down, with power-of-two block scales. Y bf16 [R,H]."""
     hq, _, h_atoms = moe_grouped_gemm_mxfp8(xq, x_atoms, w13q, w13_atoms, offsets, True, stream)
     return moe_grouped_gemm_mxfp8(hq, h_atoms, w2q, w2_atoms, offsets, False, stream)
+
+
+# ---------------------------------------------------------------------------- norm, gated feed-forward block
+def _norm_types(x, weight, *rows):
+    import torch
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError("rows [T, H] in bfloat16 or float32 expected")
+    if weight.dtype not in (x.dtype, torch.float32) or tuple(weight.shape) != (x.shape[1],):
+        raise RuntimeError("weight [H] in the type of the rows or float32 expected")
+    for r in rows:
+        if r.dtype != x.dtype or r.shape != x.shape:
+            raise RuntimeError("all rows must have one type and shape")
+    return 1 if x.dtype == torch.float32 else 0, 1 if weight.dtype == torch.float32 else 0
+
+
+def add_rms_norm(x, residual, weight, eps: float = 1e-6, r_out=None, stream=None):
+    """(y, r, rstd): r = x + residual (residual None: x itself), y = r * rstd * weight; see dk_add_rms_norm.
+    r_out: where r goes (may be residual or x itself); a new tensor by default."""
+    import torch
+    extra = [t for t in (residual, r_out) if t is not None]
+    _need_cuda(x, weight, *extra)
+    xf, wf = _norm_types(x, weight, *extra)
+    if residual is not None and r_out is None:
+        r_out = torch.empty_like(x)
+    y = torch.empty_like(x)
+    rstd = torch.empty((x.shape[0],), dtype=torch.float32, device=x.device)
+    check(lib().dk_add_rms_norm(_ptr(x), _ptr(residual) if residual is not None else None, _ptr(weight), xf, wf,
+                                x.shape[0], x.shape[1], eps, _ptr(y), _ptr(r_out) if r_out is not None else None,
+                                _ptr(rstd), _stream_ptr(stream)))
+    return y, (x if residual is None else r_out), rstd
+
+
+def add_rms_norm_mx(x, residual, weight, eps: float = 1e-6, r_out=None, stream=None):
+    """(q, s, atoms, r): add_rms_norm with y as MXFP8, laid out as mx_quant does; see dk_add_rms_norm_mx."""
+    import torch
+    extra = [t for t in (residual, r_out) if t is not None]
+    _need_cuda(x, weight, *extra)
+    xf, wf = _norm_types(x, weight, *extra)
+    if residual is not None and r_out is None:
+        r_out = torch.empty_like(x)
+    T, H = x.shape
+    u8 = dict(dtype=torch.uint8, device=x.device)
+    q, s = torch.empty((T, H), **u8), torch.empty((T, H // 32), **u8)
+    atoms = torch.empty(((T + 127) // 128, H // 128, 512), **u8)
+    check(lib().dk_add_rms_norm_mx(_ptr(x), _ptr(residual) if residual is not None else None, _ptr(weight), xf, wf, T, H,
+                                   eps, _ptr(q), _ptr(s), _ptr(atoms), _ptr(r_out) if r_out is not None else None,
+                                   _stream_ptr(stream)))
+    return q, s, atoms, (x if residual is None else r_out)
+
+
+def add_rms_norm_bwd(dy, dr, r, rstd, weight, stream=None):
+    """(dx, dw) of add_rms_norm; dx is the gradient of x and of residual. dr may be None."""
+    import torch
+    extra = [dy] + ([dr] if dr is not None else [])
+    _need_cuda(r, rstd, weight, *extra)
+    xf, wf = _norm_types(r, weight, *extra)
+    T, H = r.shape
+    if rstd.dtype != torch.float32 or rstd.numel() != T:
+        raise RuntimeError("rstd [T] in float32 expected")
+    wb = lib().dk_add_rms_norm_bwd_workspace_bytes(T, H)
+    ws = torch.empty((wb,), dtype=torch.uint8, device=r.device)
+    dx, dw = torch.empty_like(r), torch.empty_like(weight)
+    check(lib().dk_add_rms_norm_bwd(_ptr(dy), _ptr(dr) if dr is not None else None, _ptr(r), _ptr(rstd), _ptr(weight), xf,
+                                    wf, T, H, _ptr(dx), _ptr(dw), _ptr(ws), wb, _stream_ptr(stream)))
+    return dx, dw
+
+
+def _ffn_shape(x, w13, w2, *more):
+    import torch
+    _need_cuda(x, w13, w2, *more)
+    if any(t.dtype != torch.bfloat16 for t in (x, w13, w2, *more)):
+        raise RuntimeError("the gated feed-forward block expects bfloat16")
+    T, H = x.shape
+    F = w2.shape[1]
+    if tuple(w13.shape) != (2 * F, H) or w2.shape[0] != H:
+        raise RuntimeError("expected x [T,H], w13 [2F,H], w2 [H,F]")
+    return T, H, F
+
+
+def gated_ffn(x, w13, w2, save: bool = False, stream=None):
+    """y = (silu(x wg^T) * (x wu^T)) w2^T, or with save (y, gu [T,2F], h [T,F]) for gated_ffn_bwd."""
+    import torch
+    T, H, F = _ffn_shape(x, w13, w2)
+    gu = torch.empty((T, 2 * F), dtype=x.dtype, device=x.device) if save else None
+    h, y = torch.empty((T, F), dtype=x.dtype, device=x.device), torch.empty_like(x)
+    check(lib().dk_gated_ffn(_ptr(x), _ptr(w13), _ptr(w2), T, H, F, _ptr(gu) if save else None, _ptr(h), _ptr(y),
+                             _stream_ptr(stream)))
+    return (y, gu, h) if save else y
+
+
+def gated_ffn_bwd(dy, x, w13, w2, gu, h, stream=None):
+    """(dx, dw13, dw2) of gated_ffn from what it saved."""
+    import torch
+    T, H, F = _ffn_shape(x, w13, w2, dy, gu, h)
+    if dy.shape != x.shape or tuple(gu.shape) != (T, 2 * F) or tuple(h.shape) != (T, F):
+        raise RuntimeError("expected dy [T,H], gu [T,2F], h [T,F]")
+    dgu, dx, dw13, dw2 = (torch.empty_like(t) for t in (gu, x, w13, w2))
+    check(lib().dk_gated_ffn_bwd(_ptr(dy), _ptr(x), _ptr(w13), _ptr(w2), _ptr(gu), _ptr(h), T, H, F, _ptr(dgu), _ptr(dx),
+                                 _ptr(dw13), _ptr(dw2), _stream_ptr(stream)))
+    return dx, dw13, dw2
 
 
 # ---------------------------------------------------------------------------- expert parallel

@@ -1,0 +1,480 @@
+// Gated feed-forward block and its backward pass, bf16, for sm_100a.
+//
+//   [g | u] = x W13^T        x [T,H], W13 [2F,H] (F gate rows, then F up rows, as in the MoE layer)
+//   h = silu(g) * u          silu(g) = g * s, s = 1 / (1 + exp(-g))
+//   y = h W2^T               W2 [H,F]
+//
+//   dh = dy W2,  dg = dh * u * s * (1 + g * (1 - s)),  du = dh * g * s
+//   dx = [dg|du] W13,  dW13 = [dg|du]^T x,  dW2 = dy^T h
+//
+// One kernel serves all six products, D[M,N] = A B with fp32 accumulation in tensor memory. It is
+// instantiated over how the operands lie in memory: K-major ([M,K] and [N,K], the weights of a
+// forward pass) or MN-major ([K,M] and [K,N]: W2 and W13 seen from the other side, and the token axis as
+// K in the weight gradients), which the tensor core reads through a descriptor of its own, so nothing is
+// transposed in memory. What it does with a finished tile:
+//   EPI_STORE   bf16 rows of D
+//   EPI_GATED   the B tile is 128 gate rows and 128 up rows, so a thread holds g and u of the same
+//               place: silu(g) * u leaves as h, and g, u too when a backward pass will follow
+//   EPI_DGATED  D is dh: with the kept g, u of the same place, dg and du leave
+// h, g, u, dg, du are rounded to bf16, the type in which the tensor core takes them up again; silu and its
+// derivative are computed in fp32 from the accumulators (forward) or the kept bf16 values (backward).
+//
+//   warp 0      TMA producer: 128-byte-swizzled boxes into a four-stage ring
+//   warp 1      one thread issues tcgen05.mma 128x256x16 into one of two 256-column accumulators
+//   warps 2-5   epilogue: tcgen05.ld, swizzled staging in shared memory, TMA stores (which clip the
+//               ragged edges)
+#include "dk_host.h"
+#include "dk_ptx.cuh"
+
+namespace dk {
+
+namespace ffn {
+
+constexpr int BM = 128;
+constexpr int BN = 256;
+constexpr int BK = 64;  // 64 bf16 = 128 bytes = one swizzle row
+constexpr int UMMA_K = 16;
+constexpr int A_BYTES = BM * BK * 2;
+constexpr int B_BYTES = BN * BK * 2;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int STAGES = 4;
+constexpr int MN_BLOCK = 64 * BK * 2;  // an MN-major box: 64 elements of M or N (128 bytes) x 64 of K
+constexpr int EPI_BUF = 32 * 128;      // 32 rows x 64 bf16
+constexpr int EPI_BYTES = 4 * 2 * EPI_BUF;
+constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + 256;
+constexpr int THREADS = 192;
+constexpr int TMEM_COLS = 512;
+
+enum : int { EPI_STORE = 0, EPI_GATED = 1, EPI_DGATED = 2 };
+enum : unsigned { SITE_EMPTY = 101, SITE_FULL = 102, SITE_TMEM_EMPTY = 103, SITE_TMEM_FULL = 104 };
+
+struct Maps {
+    CUtensorMap a, b;
+    CUtensorMap out[3];  // STORE: D; GATED: h, g, u; DGATED: dg, du
+};
+
+struct Args {
+    int M, N, num_kb;  // N: columns of the output (GATED, DGATED: F)
+    int tiles_m, tiles_n, group_m;
+    int save;                 // GATED: g and u leave too
+    const __nv_bfloat16* gu;  // DGATED: kept [g|u], [M, 2N]
+    unsigned* status;
+};
+
+// Descriptor of an MN-major operand in boxes of 64 (M or N) x 64 (K) with the 128-byte swizzle: the
+// leading offset leads from one 64-element box to the next, the stride offset from eight K rows to
+// the next eight.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3ffff) >> 4);
+    d |= static_cast<uint64_t>(MN_BLOCK >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+
+// Column tiles run slowest inside a group of group_m row tiles, so that CTAs running together share
+// operand tiles in L2.
+__device__ __forceinline__ void tile_coords(int t, const Args& g, int& m, int& n) {
+    const int per_group = g.group_m * g.tiles_n;
+    const int grp = t / per_group;
+    const int first = grp * g.group_m;
+    const int gsz = min(g.tiles_m - first, g.group_m);
+    const int r = t - grp * per_group;
+    m = first + r % gsz;
+    n = r / gsz;
+}
+
+__device__ __forceinline__ float sigmoid_f(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
+
+// 32 packed columns (64 bytes) of this lane's row into half `hi` of a swizzled 32x64 staging buffer.
+__device__ __forceinline__ void stage_half(uint32_t buf, int lane, int hi, const uint32_t (&p)[16]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t addr = buf + lane * 128 + (((hi * 4 + j) ^ (lane & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(p[4 * j]), "r"(p[4 * j + 1]),
+                     "r"(p[4 * j + 2]), "r"(p[4 * j + 3])
+                     : "memory");
+    }
+}
+__device__ __forceinline__ void pack32(const float (&f)[32], uint32_t (&p)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+}
+__device__ __forceinline__ void ld_acc(uint32_t taddr, float (&f)[32]) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(taddr, r);
+    tmem_ld_wait(r);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+// 32 bf16 of global memory; columns at or beyond `n` (a multiple of 8) count as 0
+__device__ __forceinline__ void ld_row32(const __nv_bfloat16* p, int col, int n, bool ok, float (&f)[32]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (ok && col + 8 * j < n) v = __ldg(reinterpret_cast<const uint4*>(p + 8 * j));
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 t = __bfloat1622float2(h[i]);
+            f[8 * j + 2 * i] = t.x;
+            f[8 * j + 2 * i + 1] = t.y;
+        }
+    }
+}
+
+template <bool A_MN, bool B_MN, int EPI>
+__global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_constant__ Maps maps, const Args g) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t ring = smem_base;
+    const uint32_t epi = smem_base + STAGES * STAGE_BYTES;
+    const uint32_t ctrl = epi + EPI_BYTES;
+    uint8_t* ctrl_p = smem_raw + (ctrl - smem_u32(smem_raw));
+    const uint32_t bar_full = ctrl, bar_empty = ctrl + 8 * STAGES;
+    const uint32_t bar_tfull = ctrl + 16 * STAGES, bar_tempty = bar_tfull + 16;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl_p + 16 * STAGES + 32);
+    volatile int* abort_sm = reinterpret_cast<volatile int*>(ctrl_p + 16 * STAGES + 40);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const WaitCtx wc{g.status, abort_sm};
+    const int num_tiles = g.tiles_m * g.tiles_n;
+
+    if (threadIdx.x == 0) {
+        *abort_sm = 0;
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(bar_tfull + 8 * a, 1);
+            mbar_init(bar_tempty + 8 * a, 128);
+        }
+        fence_mbar_init();
+        tma_prefetch_desc(&maps.a);
+        tma_prefetch_desc(&maps.b);
+    }
+    if (warp == 1) {
+        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
+        tmem_relinquish<1>();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+                int m, n;
+                tile_coords(t, g, m, n);
+                for (int kb = 0; kb < g.num_kb; ++kb) {
+                    if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, wc, SITE_EMPTY, t)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t full = bar_full + 8 * s, sa = ring + s * STAGE_BYTES, sb = sa + A_BYTES;
+                    mbar_expect_tx(full, STAGE_BYTES);
+                    if (A_MN) {
+                        for (int i = 0; i < BM / 64; ++i)
+                            tma_load_2d(sa + i * MN_BLOCK, &maps.a, full, m * BM + 64 * i, kb * BK);
+                    } else {
+                        tma_load_2d(sa, &maps.a, full, kb * BK, m * BM);
+                    }
+                    if (EPI == EPI_GATED) {
+                        // gate rows that do not exist read up rows instead, up rows zeros: not stored
+                        tma_load_2d(sb, &maps.b, full, kb * BK, n * 128);
+                        tma_load_2d(sb + B_BYTES / 2, &maps.b, full, kb * BK, g.N + n * 128);
+                    } else if (B_MN) {
+                        for (int i = 0; i < BN / 64; ++i)
+                            tma_load_2d(sb + i * MN_BLOCK, &maps.b, full, n * BN + 64 * i, kb * BK);
+                    } else {
+                        tma_load_2d(sb, &maps.b, full, kb * BK, n * BN);
+                    }
+                    if (++s == STAGES) {
+                        s = 0;
+                        ph ^= 1;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = umma_idesc(1, 1, BM, BN) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+            // descriptor steps of 16 elements of K, in 16-byte units: 32 bytes along the swizzle row, or
+            // 16 rows of 128 bytes
+            constexpr uint64_t a_step = A_MN ? 16 * 128 / 16 : 2, b_step = B_MN ? 16 * 128 / 16 : 2;
+            int s = 0, acc = 0;
+            uint32_t ph = 0, acc_ph = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+                if (!mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, wc, SITE_TMEM_EMPTY, t)) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + acc * BN;
+                for (int kb = 0; kb < g.num_kb; ++kb) {
+                    if (!mbar_wait(bar_full + 8 * s, ph, wc, SITE_FULL, t)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = ring + s * STAGE_BYTES, sb = sa + A_BYTES;
+                    const uint64_t da = A_MN ? desc_mn(sa) : umma_desc_sw128(sa);
+                    const uint64_t db = B_MN ? desc_mn(sb) : umma_desc_sw128(sb);
+#pragma unroll
+                    for (int k = 0; k < BK / UMMA_K; ++k)
+                        umma_f16<1>(d_tmem, da + a_step * k, db + b_step * k, idesc, (kb | k) != 0);
+                    umma_commit<1>(bar_empty + 8 * s);
+                    if (++s == STAGES) {
+                        s = 0;
+                        ph ^= 1;
+                    }
+                }
+                if (!ok) break;
+                umma_commit<1>(bar_tfull + 8 * acc);
+                acc ^= 1;
+                if (acc == 0) acc_ph ^= 1;
+            }
+        }
+    } else {
+        const int q = warp & 3;  // TMEM lane quarter this warp may read
+        const uint32_t my_epi = epi + (warp - 2) * 2 * EPI_BUF;
+        int acc = 0, nbuf = 0;
+        uint32_t acc_ph = 0;
+        // a buffer whose last store (two stores ago) has been read
+        auto next_buf = [&]() {
+            if (lane == 0) tma_store_wait_read<1>();
+            __syncwarp();
+            return my_epi + (nbuf++ & 1) * EPI_BUF;
+        };
+        auto send = [&](uint32_t buf, const CUtensorMap* map, int col, int row) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (col < g.N && row < g.M) tma_store_2d(map, buf, col, row);
+                tma_store_commit();
+            }
+        };
+        for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+            int m, n;
+            tile_coords(t, g, m, n);
+            const int row0 = m * BM + q * 32;
+            if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, acc_ph, wc, SITE_TMEM_FULL, t))) break;
+            tc_fence_after();
+            const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+            if constexpr (EPI == EPI_STORE) {
+#pragma unroll 1
+                for (int c = 0; c < BN / 64; ++c) {
+                    const uint32_t buf = next_buf();
+#pragma unroll
+                    for (int hi = 0; hi < 2; ++hi) {
+                        float f[32];
+                        uint32_t p[16];
+                        ld_acc(t_acc + c * 64 + hi * 32, f);
+                        pack32(f, p);
+                        stage_half(buf, lane, hi, p);
+                    }
+                    send(buf, &maps.out[0], n * BN + c * 64, row0);
+                }
+            } else if constexpr (EPI == EPI_GATED) {
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    const int col = n * 128 + c * 64;
+                    if (g.save) {
+#pragma unroll 1
+                        for (int part = 0; part < 2; ++part) {  // gate, up
+                            const uint32_t buf = next_buf();
+#pragma unroll
+                            for (int hi = 0; hi < 2; ++hi) {
+                                float f[32];
+                                uint32_t p[16];
+                                ld_acc(t_acc + part * 128 + c * 64 + hi * 32, f);
+                                pack32(f, p);
+                                stage_half(buf, lane, hi, p);
+                            }
+                            send(buf, &maps.out[1 + part], col, row0);
+                        }
+                    }
+                    const uint32_t buf = next_buf();
+#pragma unroll
+                    for (int hi = 0; hi < 2; ++hi) {
+                        float gate[32], up[32];
+                        uint32_t p[16];
+                        ld_acc(t_acc + c * 64 + hi * 32, gate);
+                        ld_acc(t_acc + 128 + c * 64 + hi * 32, up);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) gate[i] = gate[i] * sigmoid_f(gate[i]) * up[i];
+                        pack32(gate, p);
+                        stage_half(buf, lane, hi, p);
+                    }
+                    send(buf, &maps.out[0], col, row0);
+                }
+            } else {
+                const int row = row0 + lane;
+                const bool row_ok = row < g.M;
+                const __nv_bfloat16* gu = g.gu + static_cast<size_t>(row) * (2 * static_cast<size_t>(g.N));
+#pragma unroll 1
+                for (int c = 0; c < BN / 64; ++c) {
+                    const int col0 = n * BN + c * 64;
+                    const uint32_t bg = next_buf();
+                    uint32_t pu[2][16];
+#pragma unroll
+                    for (int hi = 0; hi < 2; ++hi) {
+                        const int col = col0 + hi * 32;
+                        float gate[32], up[32], dh[32];
+                        ld_row32(gu + col, col, g.N, row_ok, gate);
+                        ld_row32(gu + g.N + col, col, g.N, row_ok, up);
+                        ld_acc(t_acc + c * 64 + hi * 32, dh);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float s = sigmoid_f(gate[i]);
+                            const float d = dh[i];
+                            dh[i] = d * gate[i] * s;                                          // du
+                            gate[i] = d * up[i] * s * (1.0f + gate[i] * (1.0f - s));          // dg
+                        }
+                        uint32_t pg[16];
+                        pack32(gate, pg);
+                        stage_half(bg, lane, hi, pg);
+                        pack32(dh, pu[hi]);
+                    }
+                    send(bg, &maps.out[0], col0, row0);
+                    const uint32_t bu = next_buf();
+                    stage_half(bu, lane, 0, pu[0]);
+                    stage_half(bu, lane, 1, pu[1]);
+                    send(bu, &maps.out[1], col0, row0);
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(bar_tempty + 8 * acc);
+            acc ^= 1;
+            if (acc == 0) acc_ph ^= 1;
+        }
+        if (lane == 0) tma_store_wait_all<0>();
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        if (*abort_sm) {
+            // give copies still in flight time to land before the shared memory goes away
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 200000ull) {
+            }
+        }
+        tmem_dealloc<1>(tmem_base, TMEM_COLS);
+    }
+}
+
+// --------------------------------------------------------------------------------------------
+// host side
+
+// K-major operand [rows, K] or MN-major operand [K, cols]; `box` rows of a K-major one
+static int operand_map(CUtensorMap* map, const void* p, bool mn, int rows_or_cols, int K, int box) {
+    if (mn) return make_tmap_2d(map, p, 2, rows_or_cols, K, static_cast<uint64_t>(rows_or_cols) * 2, 64, BK);
+    return make_tmap_2d(map, p, 2, K, rows_or_cols, static_cast<uint64_t>(K) * 2, BK, box);
+}
+
+template <bool A_MN, bool B_MN, int EPI>
+static int launch(const Maps& maps, const Args& g, cudaStream_t st) {
+    static bool attr_set[64] = {false};
+    int dev = 0, sms = 0;
+    DK_CUDA_OK(cudaGetDevice(&dev));
+    if (!attr_set[dev & 63]) {
+        DK_CUDA_OK(cudaFuncSetAttribute(ffn_gemm_kernel<A_MN, B_MN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        SMEM_BYTES));
+        attr_set[dev & 63] = true;
+    }
+    const int rc = sm_count(&sms);
+    if (rc != DK_OK) return rc;
+    const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
+    ffn_gemm_kernel<A_MN, B_MN, EPI><<<static_cast<int>(tiles < sms ? tiles : sms), THREADS, SMEM_BYTES, st>>>(maps, g);
+    DK_CUDA_OK(cudaGetLastError());
+    return DK_OK;
+}
+
+// D[M,N] = A B. GATED: B = W13 [2N, K], D = h. DGATED: D = dgu [M, 2N].
+template <bool A_MN, bool B_MN, int EPI>
+static int product(const void* A, const void* B, void* D, int M, int N, int K, void* gu, cudaStream_t st) {
+    Maps maps;
+    Args g{};
+    int rc = operand_map(&maps.a, A, A_MN, M, K, BM);
+    if (rc != DK_OK) return rc;
+    rc = operand_map(&maps.b, B, B_MN, EPI == EPI_GATED ? 2 * N : N, K, EPI == EPI_GATED ? 128 : BN);
+    if (rc != DK_OK) return rc;
+    const uint64_t wide = static_cast<uint64_t>(N) * 4;  // bytes of a [g|u] row
+    auto out = [&](int i, void* p, uint64_t stride) { return make_tmap_2d(&maps.out[i], p, 2, N, M, stride, 64, 32); };
+    char* const pair = static_cast<char*>(EPI == EPI_DGATED ? D : gu);
+    if (EPI == EPI_DGATED) {
+        rc = out(0, pair, wide);
+        if (rc == DK_OK) rc = out(1, pair + static_cast<size_t>(N) * 2, wide);
+    } else {
+        rc = out(0, D, static_cast<uint64_t>(N) * 2);
+        if (rc == DK_OK && EPI == EPI_GATED && gu != nullptr) rc = out(1, pair, wide);
+        if (rc == DK_OK && EPI == EPI_GATED && gu != nullptr) rc = out(2, pair + static_cast<size_t>(N) * 2, wide);
+    }
+    if (rc != DK_OK) return rc;
+    g.M = M;
+    g.N = N;
+    g.num_kb = (K + BK - 1) / BK;
+    g.tiles_m = (M + BM - 1) / BM;
+    g.tiles_n = (N + (EPI == EPI_GATED ? 128 : BN) - 1) / (EPI == EPI_GATED ? 128 : BN);
+    g.group_m = 16;
+    g.save = EPI == EPI_GATED && gu != nullptr;
+    g.gu = static_cast<const __nv_bfloat16*>(gu);
+    rc = device_status_ptr(&g.status);
+    if (rc != DK_OK) return rc;
+    return launch<A_MN, B_MN, EPI>(maps, g, st);
+}
+
+static int check_shape(int T, int H, int F) {
+    DK_REQUIRE(T >= 0, "the number of rows must not be negative");
+    DK_REQUIRE(H >= 8 && F >= 8 && H % 8 == 0 && F % 8 == 0, "H and F must be positive multiples of 8");
+    DK_REQUIRE(T <= (1 << 24) && H <= (1 << 20) && F <= (1 << 20), "at most 2^24 rows and widths of 2^20");
+    return DK_OK;
+}
+
+}  // namespace ffn
+}  // namespace dk
+
+extern "C" int dk_gated_ffn(const void* x, const void* w13, const void* w2, int T, int H, int F, void* gu, void* h, void* y,
+                            void* stream) {
+    using namespace dk;
+    using namespace dk::ffn;
+    int rc = check_shape(T, H, F);
+    if (rc != DK_OK) return rc;
+    DK_REQUIRE(w13 != nullptr && w2 != nullptr, "null operand");
+    if (T == 0) return DK_OK;
+    DK_REQUIRE(x != nullptr && h != nullptr && y != nullptr, "null operand");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    rc = product<false, false, EPI_GATED>(x, w13, h, T, F, H, gu, st);
+    if (rc != DK_OK) return rc;
+    return product<false, false, EPI_STORE>(h, w2, y, T, H, F, nullptr, st);
+}
+
+extern "C" int dk_gated_ffn_bwd(const void* dy, const void* x, const void* w13, const void* w2, const void* gu, const void* h,
+                                int T, int H, int F, void* dgu, void* dx, void* dw13, void* dw2, void* stream) {
+    using namespace dk;
+    using namespace dk::ffn;
+    int rc = check_shape(T, H, F);
+    if (rc != DK_OK) return rc;
+    DK_REQUIRE(w13 != nullptr && w2 != nullptr && dw13 != nullptr && dw2 != nullptr, "null operand");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (T == 0) {
+        DK_CUDA_OK(cudaMemsetAsync(dw13, 0, static_cast<size_t>(F) * H * 4, st));
+        DK_CUDA_OK(cudaMemsetAsync(dw2, 0, static_cast<size_t>(F) * H * 2, st));
+        return DK_OK;
+    }
+    DK_REQUIRE(dy != nullptr && x != nullptr && gu != nullptr && h != nullptr && dgu != nullptr && dx != nullptr, "null operand");
+    // dh = dy W2 (K = H, W2 [H,F] is [K,N]), straight into dg and du
+    rc = product<false, true, EPI_DGATED>(dy, w2, dgu, T, F, H, const_cast<void*>(gu), st);
+    if (rc == DK_OK) rc = product<false, true, EPI_STORE>(dgu, w13, dx, T, H, 2 * F, nullptr, st);
+    if (rc == DK_OK) rc = product<true, true, EPI_STORE>(dgu, x, dw13, 2 * F, H, T, nullptr, st);
+    if (rc == DK_OK) rc = product<true, true, EPI_STORE>(dy, h, dw2, H, F, T, nullptr, st);
+    return rc;
+}

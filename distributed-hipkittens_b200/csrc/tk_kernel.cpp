@@ -405,6 +405,246 @@ py::object moe_layer_ep(py::object X, py::object logits, int k, py::object W13q,
     return Out;
 }
 
+// ---- norm with the residual's addition, gated feed-forward block. These also run for single tokens, where
+// a kernel takes a few microseconds, so attribute names are interned and types compared by identity.
+struct Torch {
+    PyObject *tensor, *bf16, *f32, *u8, *raw_stream;
+    PyObject *s_is_contiguous, *s_is_cuda, *s_get_device, *s_shape, *s_data_ptr, *s_dtype, *s_new_empty;
+    PyObject* kw_dtype;
+    Torch() {
+        py::module_ t = py::module_::import("torch");
+        auto keep = [](py::object o) { return o.release().ptr(); };
+        tensor = keep(t.attr("Tensor"));
+        bf16 = keep(t.attr("bfloat16"));
+        f32 = keep(t.attr("float32"));
+        u8 = keep(t.attr("uint8"));
+        raw_stream = keep(py::getattr(t.attr("_C"), "_cuda_getCurrentRawStream", py::none()));
+        s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
+        s_is_cuda = PyUnicode_InternFromString("is_cuda");
+        s_get_device = PyUnicode_InternFromString("get_device");
+        s_shape = PyUnicode_InternFromString("shape");
+        s_data_ptr = PyUnicode_InternFromString("data_ptr");
+        s_dtype = PyUnicode_InternFromString("dtype");
+        s_new_empty = PyUnicode_InternFromString("new_empty");
+        kw_dtype = keep(py::make_tuple("dtype"));
+    }
+};
+const Torch& torch_api() {
+    static const Torch* t = new Torch();  // never freed: it outlives the interpreter's own teardown
+    return *t;
+}
+py::object checked(PyObject* o) {
+    if (o == nullptr) throw py::error_already_set();
+    return py::reinterpret_steal<py::object>(o);
+}
+
+// A contiguous CUDA tensor (or torch.nn.Parameter) of the current device, with at most 2 dimensions.
+struct Dense {
+    void* ptr = nullptr;
+    PyObject* dtype = nullptr;  // borrowed: torch keeps its dtypes
+    int ndim = 0;
+    int64_t shape[2] = {0, 0};
+    bool is(int64_t a) const { return ndim == 1 && shape[0] == a; }
+    bool is(int64_t a, int64_t b) const { return ndim == 2 && shape[0] == a && shape[1] == b; }
+};
+Dense dense_arg(const py::object& obj, int device, const char* name) {
+    const Torch& t = torch_api();
+    const int inst = PyObject_IsInstance(obj.ptr(), t.tensor);
+    if (inst < 0) throw py::error_already_set();
+    if (!inst) throw std::runtime_error("Expected a torch.Tensor");
+    if (checked(PyObject_CallMethodNoArgs(obj.ptr(), t.s_is_contiguous)).ptr() != Py_True)
+        throw std::runtime_error("Tensor must be contiguous");
+    if (checked(PyObject_GetAttr(obj.ptr(), t.s_is_cuda)).ptr() != Py_True)
+        throw std::runtime_error("Tensor must be on CUDA device");
+    const long on = PyLong_AsLong(checked(PyObject_CallMethodNoArgs(obj.ptr(), t.s_get_device)).ptr());
+    if (on != device)
+        throw std::runtime_error(std::string(name) + " is on cuda:" + std::to_string(on) + ", the current device is cuda:" +
+                                 std::to_string(device));
+    Dense d;
+    py::object shape = checked(PyObject_GetAttr(obj.ptr(), t.s_shape));
+    const Py_ssize_t nd = PyTuple_GET_SIZE(shape.ptr());
+    if (nd > 2) throw std::runtime_error(std::string(name) + ": expected Tensor.ndim <= 2");
+    d.ndim = static_cast<int>(nd);
+    for (Py_ssize_t i = 0; i < nd; ++i) {
+        d.shape[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape.ptr(), i));
+        if (d.shape[i] > 0x7fffffffLL) throw std::runtime_error(std::string(name) + ": a dimension passes 2^31");
+    }
+    d.dtype = checked(PyObject_GetAttr(obj.ptr(), t.s_dtype)).ptr();
+    d.ptr = PyLong_AsVoidPtr(checked(PyObject_CallMethodNoArgs(obj.ptr(), t.s_data_ptr)).ptr());
+    if (PyErr_Occurred()) throw py::error_already_set();
+    return d;
+}
+void want_dtype(const Dense& d, PyObject* dtype, const char* name, const char* what) {
+    if (d.dtype != dtype) throw std::runtime_error(std::string(name) + ": expected dtype " + what);
+}
+
+// Uninitialised tensor on the device of `like`, and its address.
+py::object new_empty(const py::object& like, int64_t rows, int64_t cols, PyObject* dtype, void** ptr) {
+    const Torch& t = torch_api();
+    py::object shape = cols < 0 ? py::object(py::make_tuple(rows)) : py::object(py::make_tuple(rows, cols));
+    PyObject* args[3] = {like.ptr(), shape.ptr(), dtype};
+    py::object o = checked(PyObject_VectorcallMethod(t.s_new_empty, args, 2, t.kw_dtype));
+    if (ptr != nullptr) *ptr = PyLong_AsVoidPtr(checked(PyObject_CallMethodNoArgs(o.ptr(), t.s_data_ptr)).ptr());
+    return o;
+}
+void* stream_of(int device) {
+    const Torch& t = torch_api();
+    if (t.raw_stream == Py_None) return current_stream();
+    py::object dev = py::int_(device);
+    return PyLong_AsVoidPtr(checked(PyObject_CallOneArg(t.raw_stream, dev.ptr())).ptr());
+}
+// On a machine without a GPU the first tensor's own check answers.
+int current_device() {
+    int dev = -1;
+    if (dk_device_get(&dev) != DK_OK) return -1;
+    return dev;
+}
+
+// What the three norm calls share: rows [T, H] in bf16 or fp32, a weight [H].
+struct NormArgs {
+    int device, T, H;
+    bool x_f32, w_f32;
+    PyObject *x_dtype, *w_dtype;
+    Dense x, res, w;
+    bool has_res;
+};
+NormArgs norm_args(const py::object& X, const py::object& Residual, const py::object& Weight, const char* x_name,
+                   const char* res_name) {
+    const Torch& t = torch_api();
+    NormArgs a;
+    a.device = current_device();
+    a.x = dense_arg(X, a.device, x_name);
+    a.w = dense_arg(Weight, a.device, "Weight");
+    a.has_res = !Residual.is_none();
+    if (a.x.ndim != 2) throw std::runtime_error(std::string(x_name) + " must be [T, H]");
+    if (a.x.dtype != t.bf16 && a.x.dtype != t.f32)
+        throw std::runtime_error(std::string(x_name) + ": expected dtype torch.bfloat16 or torch.float32");
+    a.T = static_cast<int>(a.x.shape[0]);
+    a.H = static_cast<int>(a.x.shape[1]);
+    if (!a.w.is(a.H)) throw std::runtime_error("Weight must be [H]");
+    if (a.w.dtype != a.x.dtype) want_dtype(a.w, t.f32, "Weight", "of the rows, or torch.float32");
+    if (a.has_res) {
+        a.res = dense_arg(Residual, a.device, res_name);
+        if (!a.res.is(a.T, a.H)) throw std::runtime_error(std::string(res_name) + " must be [T, H]");
+        if (a.res.dtype != a.x.dtype) throw std::runtime_error(std::string(res_name) + ": expected the dtype of the rows");
+    }
+    a.x_dtype = a.x.dtype;
+    a.w_dtype = a.w.dtype;
+    a.x_f32 = a.x.dtype == t.f32;
+    a.w_f32 = a.w.dtype == t.f32;
+    return a;
+}
+py::object stream_out(const NormArgs& a, const py::object& X, const py::object& Residual, bool inplace, void** ptr) {
+    *ptr = nullptr;
+    if (!a.has_res) {
+        if (inplace) throw std::runtime_error("inplace needs a Residual");
+        return X;
+    }
+    if (!inplace) return new_empty(X, a.T, a.H, a.x_dtype, ptr);
+    *ptr = a.res.ptr;
+    return Residual;
+}
+
+py::tuple add_rms_norm(py::object X, py::object Residual, py::object Weight, float eps, bool inplace) {
+    const Torch& t = torch_api();
+    const NormArgs a = norm_args(X, Residual, Weight, "X", "Residual");
+    void *yp, *rp, *sp;
+    py::object r = stream_out(a, X, Residual, inplace, &rp);
+    py::object y = new_empty(X, a.T, a.H, a.x_dtype, &yp);
+    py::object rstd = new_empty(X, a.T, -1, t.f32, &sp);
+    throw_on(dk_add_rms_norm(a.x.ptr, a.res.ptr, a.w.ptr, a.x_f32, a.w_f32, a.T, a.H, eps, yp, rp,
+                             static_cast<float*>(sp), stream_of(a.device)), "add_rms_norm");
+    return py::make_tuple(y, r, rstd);
+}
+
+py::tuple add_rms_norm_mx(py::object X, py::object Residual, py::object Weight, float eps, bool inplace) {
+    const Torch& t = torch_api();
+    const NormArgs a = norm_args(X, Residual, Weight, "X", "Residual");
+    if (a.H % 128 != 0) throw std::runtime_error("H must be a multiple of 128");
+    void *qp, *sp, *ap, *rp;
+    py::object r = stream_out(a, X, Residual, inplace, &rp);
+    py::object q = new_empty(X, a.T, a.H, t.u8, &qp);
+    py::object s = new_empty(X, a.T, a.H / 32, t.u8, &sp);
+    const int64_t blocks = (static_cast<int64_t>(a.T) + 127) / 128;
+    py::object flat = new_empty(X, blocks * (a.H / 128), 512, t.u8, &ap);
+    throw_on(dk_add_rms_norm_mx(a.x.ptr, a.res.ptr, a.w.ptr, a.x_f32, a.w_f32, a.T, a.H, eps, qp, sp, ap, rp,
+                                stream_of(a.device)), "add_rms_norm_mx");
+    return py::make_tuple(q, s, flat.attr("view")(blocks, a.H / 128, 512), r);
+}
+
+py::tuple add_rms_norm_bwd(py::object dY, py::object dR, py::object R, py::object rstd, py::object Weight) {
+    const Torch& t = torch_api();
+    const NormArgs a = norm_args(R, dR, Weight, "R", "dR");
+    const Dense dy = dense_arg(dY, a.device, "dY"), rs = dense_arg(rstd, a.device, "rstd");
+    if (!dy.is(a.T, a.H)) throw std::runtime_error("dY must be [T, H]");
+    if (dy.dtype != a.x_dtype) throw std::runtime_error("dY: expected the dtype of the rows");
+    if (!rs.is(a.T)) throw std::runtime_error("rstd must be [T]");
+    want_dtype(rs, t.f32, "rstd", "torch.float32");
+    const size_t wb = dk_add_rms_norm_bwd_workspace_bytes(a.T, a.H);
+    void *dxp, *dwp, *wsp;
+    py::object dx = new_empty(R, a.T, a.H, a.x_dtype, &dxp);
+    py::object dw = new_empty(R, a.H, -1, a.w_dtype, &dwp);
+    py::object ws = new_empty(R, static_cast<int64_t>(wb / 4), -1, t.f32, &wsp);
+    throw_on(dk_add_rms_norm_bwd(dy.ptr, a.res.ptr, a.x.ptr, static_cast<const float*>(rs.ptr), a.w.ptr, a.x_f32, a.w_f32,
+                                 a.T, a.H, dxp, dwp, wsp, wb, stream_of(a.device)), "add_rms_norm_bwd");
+    return py::make_tuple(dx, dw);
+}
+
+struct FfnArgs {
+    int device, T, H, F;
+    Dense x, w13, w2;
+};
+FfnArgs ffn_args(const py::object& X, const py::object& W13, const py::object& W2) {
+    const Torch& t = torch_api();
+    FfnArgs a;
+    a.device = current_device();
+    a.x = dense_arg(X, a.device, "X");
+    a.w13 = dense_arg(W13, a.device, "W13");
+    a.w2 = dense_arg(W2, a.device, "W2");
+    want_dtype(a.x, t.bf16, "X", "torch.bfloat16");
+    want_dtype(a.w13, t.bf16, "W13", "torch.bfloat16");
+    want_dtype(a.w2, t.bf16, "W2", "torch.bfloat16");
+    if (a.x.ndim != 2 || a.w2.ndim != 2) throw std::runtime_error("expected X [T,H], W13 [2F,H], W2 [H,F]");
+    a.T = static_cast<int>(a.x.shape[0]);
+    a.H = static_cast<int>(a.x.shape[1]);
+    a.F = static_cast<int>(a.w2.shape[1]);
+    if (!a.w2.is(a.H, a.F) || !a.w13.is(2 * static_cast<int64_t>(a.F), a.H))
+        throw std::runtime_error("expected X [T,H], W13 [2F,H], W2 [H,F]");
+    return a;
+}
+
+py::object gated_ffn(py::object X, py::object W13, py::object W2, bool save) {
+    const FfnArgs a = ffn_args(X, W13, W2);
+    PyObject* bf16 = a.x.dtype;
+    void *gup = nullptr, *hp, *yp;
+    py::object gu;
+    if (save) gu = new_empty(X, a.T, 2 * static_cast<int64_t>(a.F), bf16, &gup);
+    py::object h = new_empty(X, a.T, a.F, bf16, &hp);
+    py::object y = new_empty(X, a.T, a.H, bf16, &yp);
+    throw_on(dk_gated_ffn(a.x.ptr, a.w13.ptr, a.w2.ptr, a.T, a.H, a.F, gup, hp, yp, stream_of(a.device)), "gated_ffn");
+    if (save) return py::make_tuple(y, gu, h);
+    return y;
+}
+
+py::tuple gated_ffn_bwd(py::object dY, py::object X, py::object W13, py::object W2, py::object GU, py::object Hh) {
+    const FfnArgs a = ffn_args(X, W13, W2);
+    const Dense dy = dense_arg(dY, a.device, "dY"), gu = dense_arg(GU, a.device, "GU"), h = dense_arg(Hh, a.device, "H");
+    want_dtype(dy, a.x.dtype, "dY", "torch.bfloat16");
+    want_dtype(gu, a.x.dtype, "GU", "torch.bfloat16");
+    want_dtype(h, a.x.dtype, "H", "torch.bfloat16");
+    const int64_t F2 = 2 * static_cast<int64_t>(a.F);
+    if (!dy.is(a.T, a.H) || !gu.is(a.T, F2) || !h.is(a.T, a.F))
+        throw std::runtime_error("expected dY [T,H], GU [T,2F], H [T,F]");
+    void *dgup, *dxp, *dw13p, *dw2p;
+    py::object dgu = new_empty(X, a.T, F2, a.x.dtype, &dgup);
+    py::object dx = new_empty(X, a.T, a.H, a.x.dtype, &dxp);
+    py::object dw13 = new_empty(X, F2, a.H, a.x.dtype, &dw13p);
+    py::object dw2 = new_empty(X, a.H, a.F, a.x.dtype, &dw2p);
+    throw_on(dk_gated_ffn_bwd(dy.ptr, a.x.ptr, a.w13.ptr, a.w2.ptr, gu.ptr, h.ptr, a.T, a.H, a.F, dgup, dxp, dw13p, dw2p,
+                              stream_of(a.device)), "gated_ffn_bwd");
+    return py::make_tuple(dx, dw13, dw2);
+}
+
 py::tuple device_status() {
     unsigned st[4] = {0, 0, 0, 0};
     throw_on(dk_last_device_status(st), "device_status");
@@ -454,6 +694,21 @@ PYBIND11_MODULE(tk_kernel, m) {
           "2: as 1, tokens quantised per 128 channels at home and dispatched as fp8. device_epoch: the call "
           "number lives in device memory, so the call can be captured into a CUDA graph (after one eager call) "
           "and replayed, every rank the same number of times");
+    m.def("add_rms_norm", &add_rms_norm, py::arg("X"), py::arg("Residual"), py::arg("Weight"), py::arg("eps") = 1e-6f,
+          py::arg("inplace") = false,
+          "(Y, R, rstd): R = X + Residual in their type (Residual None: R is X), Y = R * rstd * Weight. bf16 or fp32 "
+          "rows [T,H], rstd fp32 [T]. inplace: R is written over Residual");
+    m.def("add_rms_norm_mx", &add_rms_norm_mx, py::arg("X"), py::arg("Residual"), py::arg("Weight"),
+          py::arg("eps") = 1e-6f, py::arg("inplace") = false,
+          "(q, s, atoms, R): add_rms_norm with Y as MXFP8, the operand of gemm_mxfp8 (see mx_quant)");
+    m.def("add_rms_norm_bwd", &add_rms_norm_bwd, py::arg("dY"), py::arg("dR"), py::arg("R"), py::arg("rstd"),
+          py::arg("Weight"), "(dX, dWeight) of add_rms_norm; dX is the gradient of X and of Residual. dR (gradient of R "
+          "from the layers above) may be None");
+    m.def("gated_ffn", &gated_ffn, py::arg("X"), py::arg("W13"), py::arg("W2"), py::arg("save") = false,
+          "Y = (silu(X Wg^T) * (X Wu^T)) W2^T, bf16: X [T,H], W13 [2F,H] (gate rows, then up rows), W2 [H,F]. "
+          "save: (Y, GU [T,2F], H [T,F]) for gated_ffn_bwd");
+    m.def("gated_ffn_bwd", &gated_ffn_bwd, py::arg("dY"), py::arg("X"), py::arg("W13"), py::arg("W2"), py::arg("GU"),
+          py::arg("H"), "(dX, dW13, dW2) of gated_ffn, from what it saved");
     m.def("device_status", &device_status,
           "(code, block, site, detail) of the first device-side wait that gave up; clears it");
 }

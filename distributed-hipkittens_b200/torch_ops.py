@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import sys
 from pathlib import Path
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -153,4 +153,160 @@ def _(x, logits, k, w13q, w13s, w2q, w2s, out, workspace, view, scale_mode=0, de
     torch._check(x.shape == out.shape and x.shape[0] == logits.shape[0], lambda: "shapes disagree")
 
 
-OPS = ("gemm", "gemm_rs", "ag_gemm", "allreduce", "mx_quant", "gemm_mxfp8", "moe_route", "moe_layer")
+# ------------------------------------------------------------------ norm, gated feed-forward block
+# The forward operators carry their gradients (torch.library.register_autograd), which are operators too.
+# Saved values (rstd, gu, h) come back as outputs that take no gradient.
+def _rows(x, weight):
+    torch._check(x.dim() == 2 and weight.dim() == 1 and x.shape[1] == weight.shape[0], lambda: "rows [T,H] and weight [H] expected")
+
+
+@torch.library.custom_op(f"{NS}::rms_norm", mutates_args=(), device_types="cuda")
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y, rstd): y = x * rstd * weight per row (tk_kernel.add_rms_norm without a residual)."""
+    y, _, rstd = _tk().add_rms_norm(x, None, weight, eps)
+    return y, rstd
+
+
+@rms_norm.register_fake
+def _(x, weight, eps=1e-6):
+    _rows(x, weight)
+    return torch.empty_like(x), x.new_empty((x.shape[0],), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NS}::add_rms_norm", mutates_args=(), device_types="cuda")
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                 eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, r, rstd): r = x + residual, y = r * rstd * weight per row (tk_kernel.add_rms_norm)."""
+    return tuple(_tk().add_rms_norm(x, residual, weight, eps))
+
+
+@add_rms_norm.register_fake
+def _(x, residual, weight, eps=1e-6):
+    _rows(x, weight)
+    torch._check(x.shape == residual.shape, lambda: "x and residual disagree")
+    return torch.empty_like(x), torch.empty_like(x), x.new_empty((x.shape[0],), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NS}::add_rms_norm_bwd", mutates_args=(), device_types="cuda")
+def add_rms_norm_bwd(dy: torch.Tensor, dr: Optional[torch.Tensor], r: torch.Tensor, rstd: torch.Tensor,
+                     weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dx, dweight) of add_rms_norm and rms_norm (tk_kernel.add_rms_norm_bwd)."""
+    return tuple(_tk().add_rms_norm_bwd(dy, dr, r, rstd, weight))
+
+
+@add_rms_norm_bwd.register_fake
+def _(dy, dr, r, rstd, weight):
+    _rows(r, weight)
+    return torch.empty_like(r), torch.empty_like(weight)
+
+
+def _rms_norm_setup(ctx, inputs, output):
+    x, weight, _ = inputs
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(x, output[1], weight)
+
+
+def _rms_norm_grad(ctx, dy, _drstd):
+    x, rstd, weight = ctx.saved_tensors
+    if dy is None:
+        return None, None, None
+    dx, dw = torch.ops.dk_b200.add_rms_norm_bwd(dy.contiguous(), None, x, rstd, weight)
+    return dx, dw, None
+
+
+rms_norm.register_autograd(_rms_norm_grad, setup_context=_rms_norm_setup)
+
+
+def _add_rms_norm_setup(ctx, inputs, output):
+    ctx.mark_non_differentiable(output[2])
+    ctx.save_for_backward(output[1], output[2], inputs[2])
+
+
+def _add_rms_norm_grad(ctx, dy, dr, _drstd):
+    r, rstd, weight = ctx.saved_tensors
+    if dy is None:
+        return dr, dr, None, None
+    dx, dw = torch.ops.dk_b200.add_rms_norm_bwd(dy.contiguous(), None if dr is None else dr.contiguous(), r, rstd, weight)
+    return dx, dx, dw, None
+
+
+add_rms_norm.register_autograd(_add_rms_norm_grad, setup_context=_add_rms_norm_setup)
+
+
+@torch.library.custom_op(f"{NS}::add_rms_norm_mx", mutates_args=(), device_types="cuda")
+def add_rms_norm_mx(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                    eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(q, s, atoms, r): add_rms_norm with y as MXFP8 (tk_kernel.add_rms_norm_mx); no gradient."""
+    return tuple(_tk().add_rms_norm_mx(x, residual, weight, eps))
+
+
+@add_rms_norm_mx.register_fake
+def _(x, residual, weight, eps=1e-6):
+    _rows(x, weight)
+    T, H = x.shape
+    torch._check(H % 128 == 0, lambda: "H must be a multiple of 128")
+    u8 = dict(dtype=torch.uint8)
+    return (x.new_empty((T, H), **u8), x.new_empty((T, H // 32), **u8),
+            x.new_empty(((T + 127) // 128, H // 128, 512), **u8), torch.empty_like(x))
+
+
+def _ffn_shapes(x, w13, w2):
+    torch._check(w13.shape[0] == 2 * w2.shape[1] and w13.shape[1] == x.shape[1] and w2.shape[0] == x.shape[1],
+                 lambda: "expected x [T,H], w13 [2F,H], w2 [H,F]")
+
+
+@torch.library.custom_op(f"{NS}::gated_ffn", mutates_args=(), device_types="cuda")
+def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> torch.Tensor:
+    """(silu(x wg^T) * (x wu^T)) w2^T, bf16 (tk_kernel.gated_ffn); no gradient: see gated_ffn_train."""
+    return _tk().gated_ffn(x, w13, w2)
+
+
+@gated_ffn.register_fake
+def _(x, w13, w2):
+    _ffn_shapes(x, w13, w2)
+    return torch.empty_like(x)
+
+
+@torch.library.custom_op(f"{NS}::gated_ffn_train", mutates_args=(), device_types="cuda")
+def gated_ffn_train(x: torch.Tensor, w13: torch.Tensor,
+                    w2: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, gu, h): gated_ffn with what its backward pass needs kept; y carries the gradient."""
+    return tuple(_tk().gated_ffn(x, w13, w2, True))
+
+
+@gated_ffn_train.register_fake
+def _(x, w13, w2):
+    _ffn_shapes(x, w13, w2)
+    T, F = x.shape[0], w2.shape[1]
+    return torch.empty_like(x), x.new_empty((T, 2 * F)), x.new_empty((T, F))
+
+
+@torch.library.custom_op(f"{NS}::gated_ffn_bwd", mutates_args=(), device_types="cuda")
+def gated_ffn_bwd(dy: torch.Tensor, x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, gu: torch.Tensor,
+                  h: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dw13, dw2) of gated_ffn_train (tk_kernel.gated_ffn_bwd)."""
+    return tuple(_tk().gated_ffn_bwd(dy, x, w13, w2, gu, h))
+
+
+@gated_ffn_bwd.register_fake
+def _(dy, x, w13, w2, gu, h):
+    _ffn_shapes(x, w13, w2)
+    return torch.empty_like(x), torch.empty_like(w13), torch.empty_like(w2)
+
+
+def _ffn_setup(ctx, inputs, output):
+    ctx.mark_non_differentiable(output[1], output[2])
+    ctx.save_for_backward(*inputs, output[1], output[2])
+
+
+def _ffn_grad(ctx, dy, _dgu, _dh):
+    if dy is None:
+        return None, None, None
+    return torch.ops.dk_b200.gated_ffn_bwd(dy.contiguous(), *ctx.saved_tensors)
+
+
+gated_ffn_train.register_autograd(_ffn_grad, setup_context=_ffn_setup)
+
+
+OPS = ("gemm", "gemm_rs", "ag_gemm", "allreduce", "mx_quant", "gemm_mxfp8", "moe_route", "moe_layer", "rms_norm",
+       "add_rms_norm", "add_rms_norm_bwd", "add_rms_norm_mx", "gated_ffn", "gated_ffn_train", "gated_ffn_bwd")

@@ -483,6 +483,54 @@ typedef struct dk_moe_ep_args {
 size_t dk_moe_ep_workspace_bytes(int T_loc, int k, int E, int H, int F, int world);
 int dk_moe_ep_layer(const dk_moe_ep_args* args, const dk_view* view, unsigned epoch, int phases, void* stream);
 
+/* ------------------------------------------------------------------ norm with the residual's addition */
+/*
+ * No counterpart in the reference's distributed path. Rows of H values, bf16 or (x_is_f32 != 0) fp32;
+ * the weight has the type of the rows or (w_is_f32 != 0) fp32. 1 <= H <= 65536, any T >= 0 (T == 0
+ * launches nothing). All sums in fp32.
+ *   r = x + residual, rounded to the type of the rows (residual == NULL: r = x, and r_out is NULL too)
+ *   y = r * rstd * weight, rstd = 1 / sqrt(mean(r^2) + eps)
+ * r_out may be the buffer of residual or of x (the stream updated in place); any other overlap of an
+ * output with an input is not allowed. A row that holds a NaN or an infinity makes NaNs in its own row only.
+ * Squares are summed in fp32: a row whose sum of squares passes 3.4e38 is normed to zeros.
+ *
+ * dk_add_rms_norm: y in the type of the rows; rstd [T] fp32 (may be NULL: not kept).
+ * dk_add_rms_norm_mx: y as MXFP8 for dk_gemm_mxfp8, as dk_mx_quant makes it from the fp32 y: q [T, H] e4m3
+ * bytes, s_rows [T, H/32], sf_atoms dk_mx_sf_bytes(T, H) bytes (rows that do not exist get 0). H % 128 == 0;
+ * q, s_rows and sf_atoms start on 16 bytes.
+ * dk_add_rms_norm_bwd: from dy, r, rstd and (may be NULL) dr, the gradient of r from the layers above:
+ * dx [T, H] (the gradient of x and of residual) and dw [H] in the type of the weight. workspace:
+ * dk_add_rms_norm_bwd_workspace_bytes(T, H) bytes, 16-byte aligned, contents undefined before and after.
+ * The same inputs give the same bits on every run on one model of GPU.
+ */
+int dk_add_rms_norm(const void* x, const void* residual, const void* weight, int x_is_f32, int w_is_f32, int T, int H,
+                    float eps, void* y, void* r_out, float* rstd, void* stream);
+int dk_add_rms_norm_mx(const void* x, const void* residual, const void* weight, int x_is_f32, int w_is_f32, int T, int H,
+                       float eps, void* q, void* s_rows, void* sf_atoms, void* r_out, void* stream);
+size_t dk_add_rms_norm_bwd_workspace_bytes(int T, int H);
+int dk_add_rms_norm_bwd(const void* dy, const void* dr, const void* r, const float* rstd, const void* weight, int x_is_f32,
+                        int w_is_f32, int T, int H, void* dx, void* dw, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* ------------------------------------------------------------------ gated feed-forward block, bf16 */
+/*
+ * No counterpart in the reference's distributed path. x [T, H], w13 [2F, H] (F gate rows, then F up rows, the
+ * layout of the MoE entry points), w2 [H, F], all bf16, rows contiguous; H and F multiples of 8.
+ *   [g | u] = x w13^T;  h = silu(g) * u  [T, F];  y = h w2^T  [T, H]
+ * dk_gated_ffn: both projections, the activation and the product in one kernel, then the down projection. h is
+ * an output and the second kernel's input; gu [T, 2F] (g, then u in every row) is written when it is not
+ * NULL. fp32 accumulation; g and u enter silu(g) * u in fp32, h, g, u and y are rounded to bf16 once. T == 0
+ * launches nothing.
+ * dk_gated_ffn_bwd: from dy and the kept gu and h: dx [T, H], dw13 [2F, H], dw2 [H, F]; dgu [T, 2F] is
+ * workspace (the gradient of gu afterwards). T == 0 clears the weight gradients.
+ * One rank of a tensor-parallel block: w13 and w2 hold its F / P inner columns, y (and dx) are then summed over
+ * the ranks with dk_allreduce.
+ */
+int dk_gated_ffn(const void* x, const void* w13, const void* w2, int T, int H, int F, void* gu, void* h, void* y,
+                 void* stream);
+int dk_gated_ffn_bwd(const void* dy, const void* x, const void* w13, const void* w2, const void* gu, const void* h, int T,
+                     int H, int F, void* dgu, void* dx, void* dw13, void* dw2, void* stream);
+
 /* ------------------------------------------------------------------ device helpers */
 /* For hosts that link this library but not the CUDA runtime (the pybind11 modules). */
 int dk_device_set(int device);

@@ -466,3 +466,40 @@ def mx_sf_atoms(s_u8: torch.Tensor) -> torch.Tensor:
     assert R % 128 == 0 and SK % 4 == 0
     t = s_u8.reshape(R // 128, 4, 32, SK // 4, 4)          # [rb, r1, r0, kb, k]
     return t.permute(0, 3, 2, 1, 4).contiguous()            # [rb, kb, r0, r1, k]
+
+
+# ---------------------------------------------------------------------------- norm, gated feed-forward block
+# In 64 bits, from the formulas. The stream r is rounded to the rows' type before the norm (it is what is kept).
+def add_rms_norm_ref(x, residual, weight, eps=1e-6):
+    """(y fp64, r in the type of x, rstd fp64)."""
+    r = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    r64 = r.double()
+    rstd = 1.0 / torch.sqrt((r64 * r64).mean(dim=1) + eps)
+    return r64 * rstd[:, None] * weight.double(), r, rstd
+
+
+def add_rms_norm_bwd_ref(dy, dr, r, rstd, weight):
+    """(dx, dw) fp64."""
+    dy, n = dy.double(), r.double() * rstd.double()[:, None]
+    g = dy * weight.double()
+    dx = rstd.double()[:, None] * (g - n * (g * n).mean(dim=1, keepdim=True))
+    return (dx if dr is None else dx + dr.double()), (dy * n).sum(dim=0)
+
+
+def gated_ffn_ref(x, w13, w2):
+    """(y, gu, h) fp64."""
+    gu = x.double() @ w13.double().t()
+    g, u = gu.chunk(2, dim=1)
+    h = g / (1.0 + torch.exp(-g)) * u
+    return h @ w2.double().t(), gu, h
+
+
+def gated_ffn_bwd_ref(dy, x, w13, w2):
+    """(dx, dw13, dw2) fp64."""
+    dy = dy.double()
+    _, gu, h = gated_ffn_ref(x, w13, w2)
+    g, u = gu.chunk(2, dim=1)
+    s = 1.0 / (1.0 + torch.exp(-g))
+    dh = dy @ w2.double()
+    dgu = torch.cat([dh * u * s * (1.0 + g * (1.0 - s)), dh * g * s], dim=1)
+    return dgu @ w13.double(), dgu.t() @ x.double(), dy.t() @ h

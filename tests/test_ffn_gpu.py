@@ -1,0 +1,344 @@
+"""gated_ffn and its backward pass against the 64-bit formulas, and the block with its norms as it is used.
+
+Tolerances. A bf16 rounding is off by at most half a step, 2^-8 relative, spread evenly: its root mean square
+is at most 2^-8 / sqrt(3) =: R of the value. Independent roundings add up in squares, and a product with
+weights that know nothing of them keeps their relative size in the 2-norm:
+  y, dw2      h and the result are rounded                                      sqrt(2) R
+  gu, h       the result is rounded                                             R
+  dx, dw13    g (its rounding enters dg and du by less than 1.25 of its size), u, dgu and the result   sqrt(4.6) R
+with 2 % on top for fp32 accumulation and the spread of a finite sample.
+
+A single value: with h = 2^-8 the largest rounding, and |.| taken of every factor,
+  g, u      e_g = K 2^-23 |x||wg|^T (fp32 accumulation of K products), + h|g| where it is kept rounded
+  h         e_h = 1.1 |u| e_g + |silu(g)| e_u + h|h|               |silu'| <= 1.1
+  y         e_h |w2|^T + (F 2^-23) |h||w2|^T + h|y|
+  dh        e_dh = H 2^-23 |dy||w2|
+  dg, du    e = 0.5 |dh||u| e_g + 1.1 |dh| e_u + 1.1 |u| e_dh + h|dg|,  1.1 |dh| e_g + |silu(g)| e_dh + h|du|     |silu''| <= 0.5
+  dx, dw13, dw2   the errors of the first factor times the second's magnitude, accumulation and rounding as for y
+and 5 % on top for products of two errors. (With few rows a weight gradient is a single product: its errors are relative to
+the value itself, not to the result's root mean square, so no bound by the latter holds.)
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+R = 2.0 ** -8 / 3 ** 0.5
+
+
+def make(T, H, F, seed=0):
+    g = torch.Generator().manual_seed(seed + T + 7 * H + 31 * F)
+    n = lambda *s, std=1.0: (torch.randn(*s, generator=g) * std).to(torch.bfloat16)
+    return n(T, H), n(2 * F, H, std=H ** -0.5), n(H, F, std=F ** -0.5), n(T, H)
+
+
+def near(got, want, roundings, tol=None, spread=1.02):
+    """`spread`: a sample of n values has a 2-norm that differs by up to about 4 / sqrt(n) from its expectation."""
+    got = got.double().to(want.device)
+    err, rms = (got - want).abs(), want.square().mean().sqrt()
+    assert err.square().mean().sqrt() <= spread * (1 + 4 / want.numel() ** 0.5) * roundings ** 0.5 * R * rms
+    if tol is not None:
+        assert (err <= 1.05 * tol + 1e-30).all()
+
+
+def bounds(x, w13, w2, dy):
+    """The largest errors of gu, h, y, dx, dw13, dw2 by the rules above."""
+    x, w13, w2, dy = (t.double() for t in (x, w13, w2, dy))
+    (T, H), F, e, u = x.shape, w2.shape[1], 2.0 ** -8, 2.0 ** -23
+    g, up = (x @ w13.t()).chunk(2, 1)
+    s = torch.sigmoid(g)
+    ag, au = (H * u * (x.abs() @ w13.abs().t())).chunk(2, 1)
+    h = g * s * up
+    eh = 1.1 * up.abs() * ag + (g * s).abs() * au + e * h.abs()
+    y = eh @ w2.abs().t() + F * u * (h.abs() @ w2.abs().t()) + e * (h @ w2.t()).abs()
+    kg, ku = ag + e * g.abs(), au + e * up.abs()
+    dh, edh = dy @ w2, H * u * (dy.abs() @ w2.abs())
+    dg, du = dh * up * (s + g * s * (1 - s)), dh * g * s
+    eg = 0.5 * (dh * up).abs() * kg + 1.1 * dh.abs() * ku + 1.1 * up.abs() * edh + e * dg.abs()
+    eu = 1.1 * dh.abs() * kg + (g * s).abs() * edh + e * du.abs()
+    d, ed = torch.cat([dg, du], 1), torch.cat([eg, eu], 1)
+    prod = lambda a, ea, b: (ea + a.shape[1] * u * a.abs()) @ b.abs() + e * (a @ b).abs()
+    return dict(gu=torch.cat([kg, ku], 1), h=eh, y=y, dx=prod(d, ed, w13), dw13=prod(d.t(), ed.t(), x),
+                dw2=prod(dy.t(), 0 * dy.t(), h) + dy.t().abs() @ eh)
+
+
+# one token to several tiles; rows and widths that end inside a tile; single vectors
+SHAPES = [(1, 512, 256), (2, 64, 64), (3, 8, 8), (5, 256, 72), (16, 1032, 136), (17, 520, 1000), (31, 2048, 4096), (33, 72, 2056),
+          (64, 4096, 512), (65, 128, 128), (100, 512, 768), (127, 136, 264), (128, 256, 256), (129, 384, 640), (200, 1024, 136),
+          (255, 264, 392), (257, 320, 1288), (513, 512, 520), (700, 2056, 1032)]
+
+
+@pytest.mark.parametrize("T,H,F", SHAPES)
+def test_forward(orc, capi, T, H, F):
+    import tk_kernel as tk
+    x, w13, w2, dy = make(T, H, F)
+    tol = bounds(*(t.cuda() for t in (x, w13, w2, dy)))
+    y64, gu64, h64 = orc.gated_ffn_ref(x.cuda(), w13.cuda(), w2.cuda())
+    y = tk.gated_ffn(x.cuda(), w13.cuda(), w2.cuda())
+    y2, gu, h = tk.gated_ffn(x.cuda(), w13.cuda(), w2.cuda(), True)
+    torch.cuda.synchronize()
+    assert capi.device_status()[0] == 0
+    near(y, y64, 2, tol["y"])
+    near(gu, gu64, 1, tol["gu"])
+    near(h, h64, 1, tol["h"])
+    assert torch.equal(y, y2)
+    assert torch.equal(tk.gated_ffn(x.cuda(), w13.cuda(), w2.cuda()), y)  # the same bits again
+
+
+@pytest.mark.parametrize("T,H,F", SHAPES)
+def test_backward(orc, capi, T, H, F):
+    import tk_kernel as tk
+    x, w13, w2, dy = (t.cuda() for t in make(T, H, F, seed=1))
+    want = orc.gated_ffn_bwd_ref(dy, x, w13, w2)
+    _, gu, h = tk.gated_ffn(x, w13, w2, True)
+    got = tk.gated_ffn_bwd(dy, x, w13, w2, gu, h)
+    torch.cuda.synchronize()
+    assert capi.device_status()[0] == 0
+    tol = bounds(x, w13, w2, dy)
+    for a, b, n, k in zip(got, want, (4.6, 4.6, 2), ("dx", "dw13", "dw2")):
+        near(a, b, n, tol[k])
+    for a, b in zip(got, tk.gated_ffn_bwd(dy, x, w13, w2, gu, h)):
+        assert torch.equal(a, b)
+
+
+def test_every_element_of_every_tile(orc):
+    """Weights that route single inputs to single outputs: each value of y is one value of x, exactly, so a tile that
+    is swapped, shifted or dropped shows. g = 32 (sigmoid(32) is 1 in fp32), u = x, h = 32 x, y = 32 x / 32."""
+    import tk_kernel as tk
+    for T, H in ((1, 512), (130, 640), (300, 264)):
+        F = H - 8
+        x = torch.randint(-64, 64, (T, H), generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
+        x[:, -1] = 1
+        w13 = torch.zeros(2 * F, H)
+        w13[:F, -1] = 32.0
+        perm = torch.randperm(F, generator=torch.Generator().manual_seed(H))
+        w13[F + torch.arange(F), perm] = 1.0
+        w2 = torch.zeros(H, F)
+        w2[torch.arange(F), torch.arange(F)] = 1 / 32
+        y = tk.gated_ffn(x.cuda(), w13.to(torch.bfloat16).cuda(), w2.to(torch.bfloat16).cuda())
+        want = torch.zeros(T, H)
+        want[:, :F] = x.float()[:, perm]
+        assert torch.equal(y.float().cpu(), want)
+
+
+def test_extreme_gates():
+    """Large gates of both signs: silu(g) is g or 0, its derivative 1 or 0, nothing turns into NaN."""
+    import tk_kernel as tk
+    T, H, F = 40, 64, 64
+    x = torch.zeros(T, H)
+    x[:, 0] = torch.linspace(-200, 200, T)
+    x[:, 1] = 1
+    w13 = torch.zeros(2 * F, H)
+    w13[:F, 0] = 4.0
+    w13[F:, 1] = 1.0
+    w2 = torch.eye(H, F)
+    x, w13, w2 = (t.to(torch.bfloat16).cuda() for t in (x, w13, w2))
+    y, gu, h = tk.gated_ffn(x, w13, w2, True)
+    dx, dw13, dw2 = tk.gated_ffn_bwd(torch.ones_like(y), x, w13, w2, gu, h)
+    g = 4 * x[:, 0].double()
+    want = g * torch.sigmoid(g)
+    assert ((h[:, 0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-30).all()
+    assert all(torch.isfinite(t.float()).all() for t in (y, dx, dw13, dw2))
+
+
+def test_non_finite_rows_stay_in_their_rows(orc):
+    import tk_kernel as tk
+    for T in (6, 300):
+        x, w13, w2, _ = make(T, 256, 136)
+        good = tk.gated_ffn(x.cuda(), w13.cuda(), w2.cuda())
+        x[2, 5] = float("nan")
+        x[4, 7] = float("inf")
+        y = tk.gated_ffn(x.cuda(), w13.cuda(), w2.cuda())
+        keep = [i for i in range(T) if i not in (2, 4)]
+        assert torch.equal(y[keep], good[keep]) and torch.isnan(y[2]).all() and not torch.isfinite(y[4]).any()
+
+
+def test_rows_do_not_depend_on_their_batch_neighbours(orc):
+    """Within one batch size a row's result depends on that row alone."""
+    import tk_kernel as tk
+    for T in (7, 150, 400):
+        x, w13, w2, _ = make(T, 512, 264)
+        a = tk.gated_ffn(x.cuda(), w13.cuda(), w2.cuda())
+        b = tk.gated_ffn(x.flip(0).contiguous().cuda(), w13.cuda(), w2.cuda())
+        assert torch.equal(a, b.flip(0))
+
+
+def test_no_rows():
+    import tk_kernel as tk
+    b = lambda *s: torch.full(s, 3.0, dtype=torch.bfloat16, device="cuda")
+    x, w13, w2 = b(0, 64), b(32, 64), b(64, 16)
+    y, gu, h = tk.gated_ffn(x, w13, w2, True)
+    assert y.shape == (0, 64) and gu.shape == (0, 32) and h.shape == (0, 16)
+    dx, dw13, dw2 = tk.gated_ffn_bwd(y, x, w13, w2, gu, h)
+    assert dx.shape == (0, 64) and (dw13 == 0).all() and (dw2 == 0).all() and dw13.shape == w13.shape and dw2.shape == w2.shape
+
+
+@pytest.mark.parametrize("T", [1, 37, 300])
+def test_nothing_is_written_outside(capi, T):
+    H, F = 136, 200
+    x, w13, w2, dy = (t.cuda() for t in make(T, H, F))
+    L, st = capi.lib(), capi._stream_ptr(None)
+    sizes = dict(gu=4 * T * F, h=2 * T * F, y=2 * T * H, dgu=4 * T * F, dx=2 * T * H, dw13=4 * F * H, dw2=2 * F * H)
+    bufs = {k: torch.full((n + 8192,), 0xA5, dtype=torch.uint8, device="cuda") for k, n in sizes.items()}
+    p = {k: b.data_ptr() + 4096 for k, b in bufs.items()}
+    capi.check(L.dk_gated_ffn(x.data_ptr(), w13.data_ptr(), w2.data_ptr(), T, H, F, p["gu"], p["h"], p["y"], st))
+    capi.check(L.dk_gated_ffn_bwd(dy.data_ptr(), x.data_ptr(), w13.data_ptr(), w2.data_ptr(), p["gu"], p["h"], T, H, F, p["dgu"],
+                                  p["dx"], p["dw13"], p["dw2"], st))
+    torch.cuda.synchronize()
+    for k, b in bufs.items():
+        assert (b[:4096] == 0xA5).all() and (b[4096 + sizes[k]:] == 0xA5).all(), k
+
+
+@pytest.mark.parametrize("T", [4, 260])
+def test_two_streams_at_once_and_graph(T):
+    """Two calls that overlap on the GPU, and a captured step replayed on other inputs."""
+    import tk_kernel as tk
+    sets = [tuple(t.cuda() for t in make(T, 1024, 512, seed=s)) for s in (1, 2)]
+
+    def step(x, w13, w2, dy):
+        y, gu, h = tk.gated_ffn(x, w13, w2, True)
+        return (y,) + tuple(tk.gated_ffn_bwd(dy, x, w13, w2, gu, h))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None, None]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = step(*sets[i])
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+    inputs = [torch.zeros_like(t) for t in sets[0]]
+    graphs = []
+    for _ in range(2):  # two graphs over the same inputs
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*inputs)
+        graphs.append((graph, out))
+    for s, w in zip(sets, want):
+        for t, v in zip(inputs, s):
+            t.copy_(v)
+        torch.cuda.synchronize()
+        for st, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(u, v) for u, v in zip(out, w))
+
+
+def test_gradients_against_differences(orc):
+    """The backward pass against central differences of the 64-bit forward along random directions."""
+    import tk_kernel as tk
+    x, w13, w2, dy = (t.cuda() for t in make(9, 128, 72, seed=3))
+    _, gu, h = tk.gated_ffn(x, w13, w2, True)
+    grads = tk.gated_ffn_bwd(dy, x, w13, w2, gu, h)
+    g = torch.Generator().manual_seed(9)
+    args = [x.double(), w13.double(), w2.double()]
+    for i, grad in enumerate(grads):
+        d = torch.randn(args[i].shape, generator=g, dtype=torch.float64).cuda() * args[i].std()
+        e = 1e-5
+        up, down = ([a + s * e * d if j == i else a for j, a in enumerate(args)] for s in (1, -1))
+        slope = ((orc.gated_ffn_ref(*up)[0] - orc.gated_ffn_ref(*down)[0]) * dy.double()).sum() / (2 * e)
+        got = (grad.double() * d).sum()
+        # the rounded gradient's error is at most sqrt(4.6) R of its norm; along d that many standard deviations of d
+        assert (got - slope).abs() <= 6 * 4.6 ** 0.5 * R * grad.double().norm() * args[i].std()
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    from distributed_hipkittens_b200 import torch_ops
+    return torch.ops.dk_b200
+
+
+def test_the_block_as_it_is_trained(ops, orc):
+    """norm with residual -> feed-forward -> added to the stream by the next norm, gradients through autograd, against
+    the same in 64 bits. Roundings on the way: the stream twice, the normed rows twice, h and y; the gradients pass
+    as many again. Each is R at most and enters once: sqrt(16) R bounds them together."""
+    T, H, F = 150, 264, 520
+    g = torch.Generator().manual_seed(4)
+    n = lambda *s, std=1.0: (torch.randn(*s, generator=g) * std).to(torch.bfloat16).cuda()
+    x, res, w13, w2, dout = n(T, H), n(T, H), n(2 * F, H, std=H ** -0.5), n(H, F, std=F ** -0.5), n(T, H)
+    wa, wb = (1 + n(H, std=0.1).float()).to(torch.bfloat16), (1 + n(H, std=0.1).float()).to(torch.bfloat16)
+    leaves = [t.clone().requires_grad_() for t in (x, res, wa, w13, w2, wb)]
+    a, r, _ = ops.add_rms_norm(leaves[0], leaves[1], leaves[2])
+    y, _, _ = ops.gated_ffn_train(a, leaves[3], leaves[4])
+    out, r2, _ = ops.add_rms_norm(y, r, leaves[5])
+    ((out * dout).sum() + r2.float().sum()).backward()
+
+    ref = [t.double().requires_grad_() for t in (x, res, wa, w13, w2, wb)]
+    norm = lambda v, w: v / torch.sqrt(v.square().mean(1, keepdim=True) + 1e-6) * w
+    s = ref[0] + ref[1]
+    a64 = norm(s, ref[2])
+    gate, up = (a64 @ ref[3].t()).chunk(2, 1)
+    y64 = (torch.nn.functional.silu(gate) * up) @ ref[4].t()
+    out64 = norm(y64 + s, ref[5])
+    ((out64 * dout.double()).sum() + (y64 + s).sum()).backward()
+    assert orc.rel_fro(out.double().cpu(), out64.detach().cpu()) <= 4 * R
+    for a, b in zip(leaves, ref):
+        assert orc.rel_fro(a.grad.double().cpu(), b.grad.cpu()) <= 4 * R
+
+
+def test_autograd_alone(ops, orc):
+    """rms_norm and gated_ffn_train with an expanded incoming gradient, and an output nobody uses."""
+    x, w13, w2, dy = (t.cuda() for t in make(20, 64, 128))
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    xr = x.clone().requires_grad_()
+    y, rstd = ops.rms_norm(xr, w)
+    assert not rstd.requires_grad
+    y.sum().backward()
+    dx64, dw64 = orc.add_rms_norm_bwd_ref(torch.ones(20, 64), None, x.cpu(), rstd.cpu(), torch.ones(64))
+    assert orc.rel_fro(w.grad.double().cpu(), dw64) <= 2.0 ** -8
+    a, r, _ = ops.add_rms_norm(xr, x, w)
+    gx, = torch.autograd.grad(r.sum(), [xr])           # only the stream is used
+    assert (gx == 1).all()
+    torch.library.opcheck(ops.rms_norm.default, (x, w.detach()), test_utils=("test_schema", "test_faketensor"))
+    torch.library.opcheck(ops.gated_ffn_train.default, (x, w13, w2), test_utils=("test_schema", "test_faketensor"))
+
+
+def test_serving_run(capi, orc):
+    """A step as it is served: norm -> feed-forward, the next norm straight into MXFP8 and its GEMM, the stream updated in
+    place; every stage against the 64-bit form of its own inputs."""
+    import tk_kernel as tk
+    for T in (1, 48, 300):
+        x, w13, w2, _ = (t.cuda() for t in make(T, 512, 768))
+        w = torch.ones(512, dtype=torch.bfloat16, device="cuda")
+        stream = x.flip(0).contiguous()
+        r_ref = (x.float() + stream.float()).to(torch.bfloat16)
+        a, r, _ = tk.add_rms_norm(x, stream, w, 1e-6, True)
+        assert r is stream and torch.equal(stream, r_ref)
+        y = tk.gated_ffn(a, w13, w2)
+        near(y, orc.gated_ffn_ref(a, w13, w2)[0], 2)
+        before = stream.clone()
+        q, s, atoms, _ = tk.add_rms_norm_mx(y, stream, w, 1e-6, True)
+        assert torch.equal(stream, (y.float() + before.float()).to(torch.bfloat16))
+        bq, bs, batoms = tk.mx_quant(w2)
+        c = tk.gemm_mxfp8(q, atoms, tk.mx_quant(w13)[0], tk.mx_quant(w13)[2], True)
+        want = orc.mx_gemm_ref(q.cpu(), s.cpu(), *(t.cpu() for t in tk.mx_quant(w13)[:2]))
+        assert orc.rel_fro(c.cpu(), want) <= 1e-5
+
+
+def test_refusals():
+    import tk_kernel as tk
+    b = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")
+    x, w13, w2 = b(4, 64), b(48, 64), b(64, 24)
+    for call, what in [
+        (lambda: tk.gated_ffn(x.float(), w13, w2), "bfloat16"),
+        (lambda: tk.gated_ffn(x, w13.half(), w2), "bfloat16"),
+        (lambda: tk.gated_ffn(x, w13[:46], w2), "expected X"),
+        (lambda: tk.gated_ffn(x, b(48, 56), w2), "expected X"),
+        (lambda: tk.gated_ffn(x, w13, b(56, 24)), "expected X"),
+        (lambda: tk.gated_ffn(x.t(), w13, w2), "contiguous"),
+        (lambda: tk.gated_ffn(x[0], w13, w2), "expected X"),
+        (lambda: tk.gated_ffn(x.cpu(), w13, w2), "CUDA device"),
+        (lambda: tk.gated_ffn(b(4, 60), b(48, 60), b(60, 24)), "multiples of 8"),
+        (lambda: tk.gated_ffn(x, b(40, 64), b(64, 20)), "multiples of 8"),
+        (lambda: tk.gated_ffn(b(4 * 64 + 4)[4:].view(4, 64), w13, w2), "16-byte"),
+        (lambda: tk.gated_ffn_bwd(b(5, 64), x, w13, w2, b(4, 48), b(4, 24)), "expected dY"),
+        (lambda: tk.gated_ffn_bwd(x, x, w13, w2, b(4, 24), b(4, 24)), "expected dY"),
+        (lambda: tk.gated_ffn_bwd(x, x, w13, w2, b(4, 48), b(4, 48)), "expected dY"),
+    ]:
+        with pytest.raises(RuntimeError, match=what):
+            call()
+    torch.cuda.synchronize()
