@@ -17,9 +17,11 @@
 #include "dk_host.h"
 #include "dk_ptx.cuh"
 
+#include <initializer_list>
+
 namespace dk {
 
-constexpr int NORM_THREADS = 256;
+constexpr int NORM_THREADS = 256;  // of the kernels that loop over wide rows
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -30,28 +32,204 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Sum over the CTA, the same value in every thread and in the same order for every launch.
-__device__ __forceinline__ float block_sum(float v) {
-    __shared__ float part[32];
+// V consecutive elements as they lie in memory: one 2- or 4-byte access, or 16-byte ones.
+template <typename T, int V>
+struct Pack {
+    static constexpr int N16 = V * static_cast<int>(sizeof(T)) / 16;  // 16-byte accesses; 0: a single element
+    static_assert(V == 1 || V * sizeof(T) % 16 == 0, "whole 16-byte vectors, or one element");
+    union {
+        uint4 v[N16 > 0 ? N16 : 1];
+        T e[V];
+    };
+    __device__ __forceinline__ Pack() {}
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (N16 > 0) {
+#pragma unroll
+            for (int i = 0; i < N16; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+            e[0] = *p;
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (N16 > 0) {
+#pragma unroll
+            for (int i = 0; i < N16; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
+        } else {
+            *p = e[0];
+        }
+    }
+    __device__ __forceinline__ void zero() {
+        if constexpr (N16 > 0) {
+#pragma unroll
+            for (int i = 0; i < N16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+            e[0] = from_f32<T>(0.f);
+        }
+    }
+};
+
+// Sum over the threads that share a row (a warp, or the CTA), the same value in every one of them and in
+// the same order on every run. `part` is used in turn by consecutive calls (which = 0, 1, 0, ...), so that one
+// barrier a call is enough: between two uses of a half lies the barrier of the other.
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int which) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();  // the last use of `part` is over
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    if constexpr (WARP) return v;
+    if ((threadIdx.x & 31) == 0) part[which][threadIdx.x >> 5] = v;
     __syncthreads();
     float s = 0.f;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) s += part[w];
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) s += part[which][w];
     return s;
 }
 
-// One CTA per row: a pass that adds, keeps r and sums the squares, and a pass that writes y. A thread
+__device__ __forceinline__ float rstd_of(float sum_sq, int H, float eps) {
+    return 1.0f / sqrtf(sum_sq / static_cast<float>(H) + eps);
+}
+// e8m0 byte of a block maximum: floor(log2(amax)) + 127 within 0..254, which is the exponent field itself
+__device__ __forceinline__ int mx_scale(float amax) { return min(static_cast<int>(__float_as_uint(amax) >> 23), 254); }
+// 2^(127 - e)
+__device__ __forceinline__ float mx_inverse(int e) {
+    return __uint_as_float(e == 254 ? 0x00400000u : static_cast<unsigned>(254 - e) << 23);
+}
+__device__ __forceinline__ size_t mx_atom_offset(int row, int group4, int KB) {
+    const int rb = row >> 7, r1 = (row & 127) >> 5, r0 = row & 31;
+    return ((static_cast<size_t>(rb) * KB + group4) * 32 + r0) * 16 + r1 * 4;
+}
+
+struct NormOut {
+    void* y;      // rows, or null with MX
+    float* rstd;  // may be null
+    uint8_t *q, *s_rows, *atoms;
+};
+
+// Rows that fit into registers: VPT vectors of V elements a thread, a row to a CTA (or to a warp where rows are
+// narrow). CTAs are persistent: the weight is read once, and the next row's loads are issued as soon as this
+// row's values have been added up, so that they are in flight during the reduction and the writing of y. Every
+// element is read once and written once.
+template <typename T, typename W, int V, int VPT, int NT, bool WARP, bool MX>
+__global__ void __launch_bounds__(NT)
+add_rms_norm_kernel(const T* x, const T* residual, const W* __restrict__ weight, int rows, int H, float eps, T* r_out,
+                    const NormOut out) {
+    __shared__ float part[2][32];
+    const int per_row = WARP ? 32 : blockDim.x;                       // threads of a row
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+    const int first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+    const int stride = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
+    const int nvec = H / V;
+    Pack<W, V> w[VPT];
+    Pack<T, V> a[VPT], b[VPT];
+    auto fetch = [&](int row) {
+        const T* xr = x + static_cast<size_t>(row) * H;
+        const T* rr = residual + static_cast<size_t>(row) * H;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int i = j * per_row + tid;
+            if (i < nvec) {
+                a[j].load(xr + static_cast<size_t>(i) * V);
+                if (residual != nullptr) b[j].load(rr + static_cast<size_t>(i) * V);
+            }
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        a[j].zero();
+        b[j].zero();
+        w[j].zero();
+    }
+    if (first < rows) fetch(first);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+        if (j * per_row + tid < nvec) w[j].load(weight + static_cast<size_t>(j * per_row + tid) * V);
+    int which = 0;
+    for (int row = first; row < rows; row += stride, which ^= 1) {
+        Pack<T, V> r[VPT];
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            r[j] = a[j];
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float v = to_f32(a[j].e[k]);
+                if (residual != nullptr) {
+                    r[j].e[k] = from_f32<T>(v + to_f32(b[j].e[k]));
+                    v = to_f32(r[j].e[k]);
+                }
+                ss += v * v;
+            }
+        }
+        if (row + stride < rows) fetch(row + stride);
+        const size_t base = static_cast<size_t>(row) * H;
+        if (residual != nullptr) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j)
+                if (j * per_row + tid < nvec) r[j].store(r_out + base + static_cast<size_t>(j * per_row + tid) * V);
+        }
+        const float rstd = rstd_of(row_sum<WARP>(ss, part, which), H, eps);
+        if (out.rstd != nullptr && tid == 0) out.rstd[row] = rstd;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int i = j * per_row + tid;
+            if constexpr (!MX) {
+                if (i < nvec) {
+                    Pack<T, V> y;
+#pragma unroll
+                    for (int k = 0; k < V; ++k) y.e[k] = from_f32<T>(to_f32(r[j].e[k]) * rstd * to_f32(w[j].e[k]));
+                    y.store(static_cast<T*>(out.y) + base + static_cast<size_t>(i) * V);
+                }
+            } else {
+                // 32 / V lanes hold a block of 32 values, 128 / V lanes the four blocks whose scale bytes are one
+                // word of s_rows and of the atoms. H % 128 == 0, so such lanes are all inside the row or all outside.
+                constexpr int BLOCK = 32 / V, WORD = 128 / V;
+                float f[V], amax = 0.f;
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    f[k] = to_f32(r[j].e[k]) * rstd * to_f32(w[j].e[k]);
+                    amax = fmaxf(amax, fabsf(f[k]));
+                }
+#pragma unroll
+                for (int o = 1; o < BLOCK; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                const int e = mx_scale(amax);
+                const float inv = mx_inverse(e);
+                uint32_t word = 0;
+                const int lane = threadIdx.x & 31, lead = lane & ~(WORD - 1);
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    word |= static_cast<uint32_t>(__shfl_sync(0xffffffffu, e, lead + g * BLOCK)) << (8 * g);
+                if (i < nvec) {
+                    uint32_t p[V / 4];
+#pragma unroll
+                    for (int k = 0; k < V / 4; ++k) {
+                        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * k] * inv, f[4 * k + 1] * inv),
+                                                                     __NV_SATFINITE, __NV_E4M3);
+                        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * k + 2] * inv, f[4 * k + 3] * inv),
+                                                                     __NV_SATFINITE, __NV_E4M3);
+                        p[k] = lo | (hi << 16);
+                    }
+                    uint8_t* dst = out.q + base + static_cast<size_t>(i) * V;
+                    if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(p[0], p[1]);
+                    else *reinterpret_cast<uint32_t*>(dst) = p[0];
+                    if (lane == lead) {
+                        const int g4 = i / WORD;
+                        *reinterpret_cast<uint32_t*>(out.s_rows + static_cast<size_t>(row) * (H / 32) + 4 * g4) = word;
+                        *reinterpret_cast<uint32_t*>(out.atoms + mx_atom_offset(row, g4, H / 128)) = word;
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Any width and alignment: a pass that adds, keeps r and sums the squares, and a pass that writes y. A thread
 // meets the same elements in both, so r_out may be the residual's or x's own buffer.
 template <typename T, typename W, bool MX>
 __global__ void __launch_bounds__(NORM_THREADS)
-add_rms_norm_kernel(const T* __restrict__ x, const T* residual, const W* __restrict__ weight, int rows, int H, float eps,
-                    T* __restrict__ y, T* r_out, float* __restrict__ rstd_out, uint8_t* __restrict__ q,
-                    uint8_t* __restrict__ s_rows, uint8_t* __restrict__ atoms) {
+add_rms_norm_wide_kernel(const T* x, const T* residual, const W* __restrict__ weight, int rows, int H, float eps, T* r_out,
+                         const NormOut out) {
+    __shared__ float part[2][32];
     constexpr int STEP = MX ? 32 : 1;  // consecutive elements of a thread
-    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    int which = 0;
+    for (int row = blockIdx.x; row < rows; row += gridDim.x, which ^= 1) {
         const size_t base = static_cast<size_t>(row) * H;
         float ss = 0.f;
         for (int c = threadIdx.x * STEP; c < H; c += NORM_THREADS * STEP)
@@ -64,55 +242,155 @@ add_rms_norm_kernel(const T* __restrict__ x, const T* residual, const W* __restr
                 }
                 ss += v * v;
             }
-        const float rstd = 1.0f / sqrtf(block_sum(ss) / static_cast<float>(H) + eps);
-        if (rstd_out != nullptr && threadIdx.x == 0) rstd_out[row] = rstd;
+        const float rstd = rstd_of(row_sum<false>(ss, part, which), H, eps);
+        if (out.rstd != nullptr && threadIdx.x == 0) out.rstd[row] = rstd;
         const T* r = residual != nullptr ? r_out : x;
         for (int c = threadIdx.x * STEP; c < H; c += NORM_THREADS * STEP) {
             if constexpr (!MX) {
-                y[base + c] = from_f32<T>(to_f32(r[base + c]) * rstd * to_f32(weight[c]));
+                static_cast<T*>(out.y)[base + c] = from_f32<T>(to_f32(r[base + c]) * rstd * to_f32(weight[c]));
             } else {
                 float amax = 0.f;
                 for (int i = 0; i < 32; ++i)
                     amax = fmaxf(amax, fabsf(to_f32(r[base + c + i]) * rstd * to_f32(weight[c + i])));
-                int e = 0;
-                if (amax != 0.f) {
-                    int ex;
-                    (void)frexpf(amax, &ex);
-                    e = min(max(ex - 1 + 127, 0), 254);
-                }
-                const float inv = ldexpf(1.0f, 127 - e);
+                const int e = mx_scale(amax);
+                const float inv = mx_inverse(e);
                 for (int i = 0; i < 32; ++i)
-                    q[base + c + i] = __nv_cvt_float_to_fp8(to_f32(r[base + c + i]) * rstd * to_f32(weight[c + i]) * inv,
-                                                            __NV_SATFINITE, __NV_E4M3);
+                    out.q[base + c + i] = __nv_cvt_float_to_fp8(to_f32(r[base + c + i]) * rstd * to_f32(weight[c + i]) * inv,
+                                                                __NV_SATFINITE, __NV_E4M3);
                 const int kg = c >> 5;
-                s_rows[static_cast<size_t>(row) * (H / 32) + kg] = static_cast<uint8_t>(e);
-                const int rb = row >> 7, r1 = (row & 127) >> 5, r0 = row & 31;
-                atoms[((static_cast<size_t>(rb) * (H / 128) + (kg >> 2)) * 32 + r0) * 16 + r1 * 4 + (kg & 3)] =
-                    static_cast<uint8_t>(e);
+                out.s_rows[static_cast<size_t>(row) * (H / 32) + kg] = static_cast<uint8_t>(e);
+                out.atoms[mx_atom_offset(row, kg >> 2, H / 128) + (kg & 3)] = static_cast<uint8_t>(e);
             }
         }
     }
 }
 
-// A CTA takes every gridDim.x-th row and sums its share of dw in its row of `partial`
-// [gridDim.x][H], each element by one thread in row order: the same bits on every run.
-template <typename T, typename W>
-__global__ void __launch_bounds__(NORM_THREADS)
+// Backward pass on the same plan: the row's dy, r and dr in registers, the next row's on their way, and the
+// thread's columns of dw summed in registers over the CTA's rows. Each CTA leaves one row of `partial`
+// [gridDim.x][H]; every element is summed by one thread in row order: the same bits on every run.
+template <typename T, typename W, int V, int VPT, int NT, bool WARP>
+__global__ void __launch_bounds__(NT)
 add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, const T* __restrict__ r,
                         const float* __restrict__ rstd_in, const W* __restrict__ weight, int rows, int H,
                         T* __restrict__ dx, float* __restrict__ partial) {
+    __shared__ float part[2][32];
+    __shared__ float warp_dw[WARP ? NT / 32 : 1][WARP ? 32 * VPT * V : 1];
+    const int per_row = WARP ? 32 : blockDim.x;
+    const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
+    const int first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+    const int stride = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
+    const int nvec = H / V;
+    Pack<W, V> w[VPT];
+    Pack<T, V> a[VPT], b[VPT], c[VPT];
+    float next_rstd = 0.f;
+    float dw[VPT][V];
+    auto fetch = [&](int row) {
+        const size_t base = static_cast<size_t>(row) * H;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int i = j * per_row + tid;
+            if (i < nvec) {
+                a[j].load(dy + base + static_cast<size_t>(i) * V);
+                b[j].load(r + base + static_cast<size_t>(i) * V);
+            }
+        }
+        next_rstd = rstd_in[row];
+    };
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        a[j].zero();
+        b[j].zero();
+        c[j].zero();
+        w[j].zero();
+#pragma unroll
+        for (int k = 0; k < V; ++k) dw[j][k] = 0.f;
+    }
+    if (first < rows) fetch(first);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+        if (j * per_row + tid < nvec) w[j].load(weight + static_cast<size_t>(j * per_row + tid) * V);
+    int which = 0;
+    for (int row = first; row < rows; row += stride, which ^= 1) {
+        const size_t base = static_cast<size_t>(row) * H;
+        const float rstd = next_rstd;
+        if (dr != nullptr) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j)
+                if (j * per_row + tid < nvec) c[j].load(dr + base + static_cast<size_t>(j * per_row + tid) * V);
+        }
+        Pack<T, V> d[VPT], h[VPT];
+        float dot = 0.f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            d[j] = a[j];
+            h[j] = b[j];
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float dn = to_f32(d[j].e[k]) * (to_f32(h[j].e[k]) * rstd);
+                dot += dn * to_f32(w[j].e[k]);
+                dw[j][k] += dn;
+            }
+        }
+        if (row + stride < rows) fetch(row + stride);
+        const float mean = row_sum<WARP>(dot, part, which) / static_cast<float>(H);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int i = j * per_row + tid;
+            if (i < nvec) {
+                Pack<T, V> o;
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float n = to_f32(h[j].e[k]) * rstd;
+                    float v = rstd * (to_f32(d[j].e[k]) * to_f32(w[j].e[k]) - n * mean);
+                    if (dr != nullptr) v += to_f32(c[j].e[k]);
+                    o.e[k] = from_f32<T>(v);
+                }
+                o.store(dx + base + static_cast<size_t>(i) * V);
+            }
+        }
+    }
+    float* mine = partial + static_cast<size_t>(blockIdx.x) * H;
+    if constexpr (WARP) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+#pragma unroll
+            for (int k = 0; k < V; ++k) warp_dw[threadIdx.x >> 5][(j * 32 + tid) * V + k] = dw[j][k];
+        __syncthreads();
+        for (int col = threadIdx.x; col < H; col += blockDim.x) {
+            float s = 0.f;
+            for (int q = 0; q < NT / 32; ++q) s += warp_dw[q][col];
+            mine[col] = s;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+            if (j * per_row + tid < nvec) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) mine[static_cast<size_t>(j * per_row + tid) * V + k] = dw[j][k];
+            }
+    }
+}
+
+// Any width and alignment.
+template <typename T, typename W>
+__global__ void __launch_bounds__(NORM_THREADS)
+add_rms_norm_bwd_wide_kernel(const T* __restrict__ dy, const T* __restrict__ dr, const T* __restrict__ r,
+                             const float* __restrict__ rstd_in, const W* __restrict__ weight, int rows, int H,
+                             T* __restrict__ dx, float* __restrict__ partial) {
+    __shared__ float part[2][32];
     float* mine = partial + static_cast<size_t>(blockIdx.x) * H;
     for (int c = threadIdx.x; c < H; c += NORM_THREADS) mine[c] = 0.f;
-    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    int which = 0;
+    for (int row = blockIdx.x; row < rows; row += gridDim.x, which ^= 1) {
         const size_t base = static_cast<size_t>(row) * H;
         const float rstd = rstd_in[row];
         float dot = 0.f;
         for (int c = threadIdx.x; c < H; c += NORM_THREADS) {
-            const float n = to_f32(r[base + c]) * rstd, d = to_f32(dy[base + c]);
-            dot += d * to_f32(weight[c]) * n;
-            mine[c] += d * n;
+            const float dn = to_f32(dy[base + c]) * (to_f32(r[base + c]) * rstd);
+            dot += dn * to_f32(weight[c]);
+            mine[c] += dn;
         }
-        const float mean = block_sum(dot) / static_cast<float>(H);
+        const float mean = row_sum<false>(dot, part, which) / static_cast<float>(H);
         for (int c = threadIdx.x; c < H; c += NORM_THREADS) {
             const float n = to_f32(r[base + c]) * rstd;
             float v = rstd * (to_f32(dy[base + c]) * to_f32(weight[c]) - n * mean);
@@ -122,22 +400,36 @@ add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, cons
     }
 }
 
-// dw[c] = sum of the CTAs' partial sums, in their order.
+// dw[c] = sum of the CTAs' partial sums: 32 columns to a CTA, its eight warps each take every eighth part, and
+// their sums are added up in order.
 template <typename W>
-__global__ void __launch_bounds__(NORM_THREADS)
+__global__ void __launch_bounds__(256)
 add_rms_norm_dw_kernel(const float* __restrict__ partial, int parts, int H, W* __restrict__ dw) {
-    const int c = blockIdx.x * NORM_THREADS + threadIdx.x;
-    if (c >= H) return;
+    __shared__ float sum[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + lane;
     float s = 0.f;
-    for (int p = 0; p < parts; ++p) s += partial[static_cast<size_t>(p) * H + c];
-    dw[c] = from_f32<W>(s);
+    if (c < H) {
+#pragma unroll 4
+        for (int p = warp; p < parts; p += 8) s += partial[static_cast<size_t>(p) * H + c];
+    }
+    sum[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && c < H) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v += sum[q][lane];
+        dw[c] = from_f32<W>(v);
+    }
 }
 
 // --------------------------------------------------------------------------------------------
 // host side
 
 constexpr int NORM_MAX_H = 65536;
-constexpr int NORM_BWD_PARTS = 296;  // CTAs of the backward pass at most: two per SM
+constexpr int NORM_MAX_SMS = 160;
+// rows of `partial` at most: CTAs of a backward pass
+constexpr int NORM_BWD_PARTS = 2 * NORM_MAX_SMS;
 
 static int check_norm(const void* x, const void* weight, int x_is_f32, int w_is_f32, int T, int H) {
     DK_REQUIRE(T >= 0, "the number of rows must not be negative");
@@ -147,21 +439,120 @@ static int check_norm(const void* x, const void* weight, int x_is_f32, int w_is_
     return DK_OK;
 }
 
+// How a pass over T rows of H elements is cut up.
+//   vec      16-byte accesses: every row and the weight start on 16 bytes
+//   few      at most one row for each SM: as many threads to a row as it can use (latency); otherwise four
+//            vectors a thread, so that a CTA has enough bytes in flight (bandwidth)
+//   warp     rows of at most 4 vectors (or 8 elements) a lane: a row to a warp, no barrier
+//   wide     a row that does not fit into the registers of 512 threads
+enum class NormPlan { VEC_FEW, VEC_FEW2, VEC_MANY, VEC_MANY512, VEC_WARP, ONE_FEW, ONE_MANY, ONE_WARP, WIDE };
+static NormPlan norm_plan(bool vec, int V, int T, int H, int sms) {
+    const int n = vec ? H / V : H;
+    const bool few = T <= sms;
+    if (vec) {
+        if (!few && n <= 128) return NormPlan::VEC_WARP;
+        if (few && n <= 1024) return NormPlan::VEC_FEW;
+        if (few && n <= 2048) return NormPlan::VEC_FEW2;
+        if (n <= 1024) return NormPlan::VEC_MANY;
+        return n <= 2048 ? NormPlan::VEC_MANY512 : NormPlan::WIDE;
+    }
+    if (!few && n <= 256) return NormPlan::ONE_WARP;
+    if (n > 8192) return NormPlan::WIDE;
+    return few ? NormPlan::ONE_FEW : NormPlan::ONE_MANY;
+}
+static int round_threads(int n, int vpt) { return ((n + vpt - 1) / vpt + 31) / 32 * 32; }
+static bool aligned16(std::initializer_list<const void*> ps) {
+    uintptr_t bits = 0;
+    for (const void* p : ps) bits |= reinterpret_cast<uintptr_t>(p);
+    return (bits & 15) == 0;
+}
+
+template <typename T, typename W, bool MX>
+static int launch_norm(const void* x, const void* residual, const void* weight, int rows, int H, float eps, void* r_out,
+                       const NormOut& out, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc != DK_OK) return rc;
+    const bool vec = H % V == 0 && aligned16({x, residual, weight, r_out, out.y});
+    const NormPlan plan = norm_plan(vec, V, rows, H, sms);
+    const int n = vec ? H / V : H;
+    auto go = [&](auto kernel, int threads, int rows_per_cta, int ctas_per_sm) {
+        const int need = (rows + rows_per_cta - 1) / rows_per_cta, most = sms * ctas_per_sm;
+        kernel<<<need < most ? need : most, threads, 0, st>>>(static_cast<const T*>(x), static_cast<const T*>(residual),
+                                                              static_cast<const W*>(weight), rows, H, eps,
+                                                              static_cast<T*>(r_out), out);
+    };
+    switch (plan) {
+        case NormPlan::VEC_FEW: go(add_rms_norm_kernel<T, W, V, 1, 1024, false, MX>, round_threads(n, 1), 1, 1); break;
+        case NormPlan::VEC_FEW2: go(add_rms_norm_kernel<T, W, V, 2, 1024, false, MX>, round_threads(n, 2), 1, 1); break;
+        case NormPlan::VEC_MANY: {
+            const int threads = round_threads(n, 4);
+            go(add_rms_norm_kernel<T, W, V, 4, 256, false, MX>, threads, 1, 512 / threads);
+            break;
+        }
+        case NormPlan::VEC_MANY512: go(add_rms_norm_kernel<T, W, V, 4, 512, false, MX>, round_threads(n, 4), 1, 1); break;
+        case NormPlan::VEC_WARP: go(add_rms_norm_kernel<T, W, V, 4, 256, true, MX>, 256, 8, 2); break;
+        default:
+            if constexpr (!MX) {
+                if (plan == NormPlan::ONE_FEW) {
+                    go(add_rms_norm_kernel<T, W, 1, 8, 1024, false, false>, round_threads(n, 8), 1, 1);
+                    break;
+                }
+                if (plan == NormPlan::ONE_MANY) {
+                    go(add_rms_norm_kernel<T, W, 1, 16, 512, false, false>, round_threads(n, 16), 1,
+                       1024 / round_threads(n, 16));
+                    break;
+                }
+                if (plan == NormPlan::ONE_WARP) {
+                    go(add_rms_norm_kernel<T, W, 1, 8, 256, true, false>, 256, 8, 4);
+                    break;
+                }
+            }
+            go(add_rms_norm_wide_kernel<T, W, MX>, NORM_THREADS, 1, 8);
+    }
+    DK_CUDA_OK(cudaGetLastError());
+    return DK_OK;
+}
 template <bool MX>
 static int launch_norm(const void* x, const void* residual, const void* weight, int x_is_f32, int w_is_f32, int T, int H,
-                       float eps, void* y, void* r_out, float* rstd, void* q, void* s_rows, void* atoms, cudaStream_t st) {
-    const int grid = T < (1 << 20) ? T : (1 << 20);
-    auto go = [&](auto tx, auto tw) {
-        using TX = decltype(tx);
-        using TW = decltype(tw);
-        add_rms_norm_kernel<TX, TW, MX><<<grid, NORM_THREADS, 0, st>>>(
-            static_cast<const TX*>(x), static_cast<const TX*>(residual), static_cast<const TW*>(weight), T, H, eps,
-            static_cast<TX*>(y), static_cast<TX*>(r_out), rstd, static_cast<uint8_t*>(q), static_cast<uint8_t*>(s_rows),
-            static_cast<uint8_t*>(atoms));
+                       float eps, void* r_out, const NormOut& out, cudaStream_t st) {
+    if (x_is_f32) return launch_norm<float, float, MX>(x, residual, weight, T, H, eps, r_out, out, st);
+    if (w_is_f32) return launch_norm<__nv_bfloat16, float, MX>(x, residual, weight, T, H, eps, r_out, out, st);
+    return launch_norm<__nv_bfloat16, __nv_bfloat16, MX>(x, residual, weight, T, H, eps, r_out, out, st);
+}
+
+template <typename T, typename W>
+static int launch_norm_bwd(const void* dy, const void* dr, const void* r, const float* rstd, const void* weight, int rows,
+                           int H, void* dx, void* dw, float* partial, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc != DK_OK) return rc;
+    if (sms > NORM_MAX_SMS) sms = NORM_MAX_SMS;
+    const bool vec = H % V == 0 && aligned16({dy, dr, r, weight, dx});
+    const NormPlan plan = norm_plan(vec, V, rows, H, sms);
+    const int n = vec ? H / V : H;
+    int parts = 0;
+    auto go = [&](auto kernel, int threads, int rows_per_cta, int ctas_per_sm) {
+        const int need = (rows + rows_per_cta - 1) / rows_per_cta, most = sms * (ctas_per_sm < 2 ? ctas_per_sm : 2);
+        parts = need < most ? need : most;
+        kernel<<<parts, threads, 0, st>>>(static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r),
+                                          rstd, static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial);
     };
-    if (x_is_f32) go(float{}, float{});
-    else if (w_is_f32) go(__nv_bfloat16{}, float{});
-    else go(__nv_bfloat16{}, __nv_bfloat16{});
+    switch (plan) {
+        case NormPlan::VEC_FEW: go(add_rms_norm_bwd_kernel<T, W, V, 1, 1024, false>, round_threads(n, 1), 1, 1); break;
+        case NormPlan::VEC_FEW2: go(add_rms_norm_bwd_kernel<T, W, V, 2, 1024, false>, round_threads(n, 2), 1, 1); break;
+        case NormPlan::VEC_MANY: go(add_rms_norm_bwd_kernel<T, W, V, 4, 256, false>, round_threads(n, 4), 1, 1); break;
+        case NormPlan::VEC_MANY512: go(add_rms_norm_bwd_kernel<T, W, V, 4, 512, false>, round_threads(n, 4), 1, 1); break;
+        case NormPlan::VEC_WARP: go(add_rms_norm_bwd_kernel<T, W, V, 4, 256, true>, 256, 8, 2); break;
+        case NormPlan::ONE_FEW: go(add_rms_norm_bwd_kernel<T, W, 1, 8, 1024, false>, round_threads(n, 8), 1, 1); break;
+        case NormPlan::ONE_MANY: go(add_rms_norm_bwd_kernel<T, W, 1, 16, 512, false>, round_threads(n, 16), 1, 2); break;
+        case NormPlan::ONE_WARP: go(add_rms_norm_bwd_kernel<T, W, 1, 8, 256, true>, 256, 8, 2); break;
+        case NormPlan::WIDE: go(add_rms_norm_bwd_wide_kernel<T, W>, NORM_THREADS, 1, 2); break;
+    }
+    DK_CUDA_OK(cudaGetLastError());
+    add_rms_norm_dw_kernel<W><<<(H + 31) / 32, 256, 0, st>>>(partial, parts, H, static_cast<W*>(dw));
     DK_CUDA_OK(cudaGetLastError());
     return DK_OK;
 }
@@ -177,8 +568,8 @@ extern "C" int dk_add_rms_norm(const void* x, const void* residual, const void* 
     if (T == 0) return DK_OK;
     DK_REQUIRE(y != nullptr, "null output");
     DK_REQUIRE((residual != nullptr) == (r_out != nullptr), "r_out goes with a residual, and a residual with r_out");
-    return launch_norm<false>(x, residual, weight, x_is_f32, w_is_f32, T, H, eps, y, r_out, rstd, nullptr, nullptr, nullptr,
-                              static_cast<cudaStream_t>(stream));
+    return launch_norm<false>(x, residual, weight, x_is_f32, w_is_f32, T, H, eps, r_out,
+                              NormOut{y, rstd, nullptr, nullptr, nullptr}, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dk_add_rms_norm_mx(const void* x, const void* residual, const void* weight, int x_is_f32, int w_is_f32, int T,
@@ -197,7 +588,9 @@ extern "C" int dk_add_rms_norm_mx(const void* x, const void* residual, const voi
     if (T % 128 != 0)
         DK_CUDA_OK(cudaMemsetAsync(static_cast<uint8_t*>(sf_atoms) + static_cast<size_t>(T / 128) * (H / 128) * 512, 0,
                                    static_cast<size_t>(H / 128) * 512, static_cast<cudaStream_t>(stream)));
-    return launch_norm<true>(x, residual, weight, x_is_f32, w_is_f32, T, H, eps, nullptr, r_out, nullptr, q, s_rows, sf_atoms,
+    return launch_norm<true>(x, residual, weight, x_is_f32, w_is_f32, T, H, eps, r_out,
+                             NormOut{nullptr, nullptr, static_cast<uint8_t*>(q), static_cast<uint8_t*>(s_rows),
+                                     static_cast<uint8_t*>(sf_atoms)},
                              static_cast<cudaStream_t>(stream));
 }
 
@@ -223,20 +616,8 @@ extern "C" int dk_add_rms_norm_bwd(const void* dy, const void* dr, const void* r
     DK_REQUIRE(dx != nullptr, "null output");
     DK_REQUIRE(workspace != nullptr && workspace_bytes >= dk_add_rms_norm_bwd_workspace_bytes(T, H), "workspace too small");
     DK_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "the workspace must be 16-byte aligned");
-    const int parts = T < NORM_BWD_PARTS ? T : NORM_BWD_PARTS;
     float* partial = static_cast<float*>(workspace);
-    auto go = [&](auto tx, auto tw) {
-        using TX = decltype(tx);
-        using TW = decltype(tw);
-        add_rms_norm_bwd_kernel<TX, TW><<<parts, NORM_THREADS, 0, st>>>(
-            static_cast<const TX*>(dy), static_cast<const TX*>(dr), static_cast<const TX*>(r), rstd,
-            static_cast<const TW*>(weight), T, H, static_cast<TX*>(dx), partial);
-        add_rms_norm_dw_kernel<TW><<<(H + NORM_THREADS - 1) / NORM_THREADS, NORM_THREADS, 0, st>>>(partial, parts, H,
-                                                                                                  static_cast<TW*>(dw));
-    };
-    if (x_is_f32) go(float{}, float{});
-    else if (w_is_f32) go(__nv_bfloat16{}, float{});
-    else go(__nv_bfloat16{}, __nv_bfloat16{});
-    DK_CUDA_OK(cudaGetLastError());
-    return DK_OK;
+    if (x_is_f32) return launch_norm_bwd<float, float>(dy, dr, r, rstd, weight, T, H, dx, dw, partial, st);
+    if (w_is_f32) return launch_norm_bwd<__nv_bfloat16, float>(dy, dr, r, rstd, weight, T, H, dx, dw, partial, st);
+    return launch_norm_bwd<__nv_bfloat16, __nv_bfloat16>(dy, dr, r, rstd, weight, T, H, dx, dw, partial, st);
 }
