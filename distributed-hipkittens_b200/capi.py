@@ -586,10 +586,10 @@ def _ffn_shape(x, w13, w2, *more):
 
 
 def gated_ffn(x, w13, w2, save: bool = False, stream=None):
-    """y = (silu(x wg^T) * (x wu^T)) w2^T, or with save (y, gu [T,2F], h [T,F]) for gated_ffn_bwd."""
+    """y = (silu(x wg^T) * (x wu^T)) w2^T, or with save (y, gu fp32 [T,2F], h [T,F]) for gated_ffn_bwd."""
     import torch
     T, H, F = _ffn_shape(x, w13, w2)
-    gu = torch.empty((T, 2 * F), dtype=x.dtype, device=x.device) if save else None
+    gu = torch.empty((T, 2 * F), dtype=torch.float32, device=x.device) if save else None
     h, y = torch.empty((T, F), dtype=x.dtype, device=x.device), torch.empty_like(x)
     check(lib().dk_gated_ffn(_ptr(x), _ptr(w13), _ptr(w2), T, H, F, _ptr(gu) if save else None, _ptr(h), _ptr(y),
                              _stream_ptr(stream)))
@@ -599,10 +599,12 @@ def gated_ffn(x, w13, w2, save: bool = False, stream=None):
 def gated_ffn_bwd(dy, x, w13, w2, gu, h, stream=None):
     """(dx, dw13, dw2) of gated_ffn from what it saved."""
     import torch
-    T, H, F = _ffn_shape(x, w13, w2, dy, gu, h)
-    if dy.shape != x.shape or tuple(gu.shape) != (T, 2 * F) or tuple(h.shape) != (T, F):
-        raise RuntimeError("expected dy [T,H], gu [T,2F], h [T,F]")
-    dgu, dx, dw13, dw2 = (torch.empty_like(t) for t in (gu, x, w13, w2))
+    T, H, F = _ffn_shape(x, w13, w2, dy, h)
+    _need_cuda(gu)
+    if dy.shape != x.shape or tuple(gu.shape) != (T, 2 * F) or tuple(h.shape) != (T, F) or gu.dtype != torch.float32:
+        raise RuntimeError("expected dy [T,H], gu [T,2F] (float32), h [T,F]")
+    dx, dw13, dw2 = (torch.empty_like(t) for t in (x, w13, w2))
+    dgu = torch.empty_like(gu, dtype=x.dtype)
     check(lib().dk_gated_ffn_bwd(_ptr(dy), _ptr(x), _ptr(w13), _ptr(w2), _ptr(gu), _ptr(h), T, H, F, _ptr(dgu), _ptr(dx),
                                  _ptr(dw13), _ptr(dw2), _stream_ptr(stream)))
     return dx, dw13, dw2

@@ -16,8 +16,10 @@
 //   EPI_GATED   the B tile is 128 gate rows and 128 up rows, so a thread holds g and u of the same
 //               place: silu(g) * u leaves as h, and g, u too when a backward pass will follow
 //   EPI_DGATED  D is dh: with the kept g, u of the same place, dg and du leave
-// h, g, u, dg, du are rounded to bf16, the type in which the tensor core takes them up again; silu and its
-// derivative are computed in fp32 from the accumulators (forward) or the kept bf16 values (backward).
+// h, dg and du are rounded to bf16, the type in which the tensor core takes them up again. g and u are kept in
+// 32 bits: dx and dW13 then carry two roundings, [dg|du] and their own (error against 64 bits 0.0024); kept in bf16
+// their roundings entered too (0.0030). The price is 8 bytes a value of h instead of 4, written and read beside
+// matrix products.
 //
 //   warp 0      TMA producer: 128-byte-swizzled boxes into a four-stage ring
 //   warp 1      one thread issues tcgen05.mma 128x256x16 into one of two 256-column accumulators
@@ -57,7 +59,7 @@ struct Args {
     int M, N, num_kb;  // N: columns of the output (GATED, DGATED: F)
     int tiles_m, tiles_n, group_m;
     int save;                 // GATED: g and u leave too
-    const __nv_bfloat16* gu;  // DGATED: kept [g|u], [M, 2N]
+    const float* gu;          // DGATED: kept [g|u], [M, 2N]
     unsigned* status;
 };
 
@@ -109,19 +111,16 @@ __device__ __forceinline__ void ld_acc(uint32_t taddr, float (&f)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
 }
-// 32 bf16 of global memory; columns at or beyond `n` (a multiple of 8) count as 0
-__device__ __forceinline__ void ld_row32(const __nv_bfloat16* p, int col, int n, bool ok, float (&f)[32]) {
+// 32 fp32 of global memory; columns at or beyond `n` (a multiple of 8) count as 0
+__device__ __forceinline__ void ld_row32(const float* p, int col, int n, bool ok, float (&f)[32]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (ok && col + 8 * j < n) v = __ldg(reinterpret_cast<const uint4*>(p + 8 * j));
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 t = __bfloat1622float2(h[i]);
-            f[8 * j + 2 * i] = t.x;
-            f[8 * j + 2 * i + 1] = t.y;
-        }
+    for (int j = 0; j < 8; ++j) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ok && col + 4 * j < n) v = __ldg(reinterpret_cast<const float4*>(p) + j);
+        f[4 * j] = v.x;
+        f[4 * j + 1] = v.y;
+        f[4 * j + 2] = v.z;
+        f[4 * j + 3] = v.w;
     }
 }
 
@@ -251,11 +250,12 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
             __syncwarp();
             return my_epi + (nbuf++ & 1) * EPI_BUF;
         };
-        auto send = [&](uint32_t buf, const CUtensorMap* map, int col, int row) {
+        // `words`: bf16 units an element takes up (the maps count in those)
+        auto send = [&](uint32_t buf, const CUtensorMap* map, int col, int row, int words = 1) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-                if (col < g.N && row < g.M) tma_store_2d(map, buf, col, row);
+                if (col < g.N && row < g.M) tma_store_2d(map, buf, col * words, row);
                 tma_store_commit();
             }
         };
@@ -286,17 +286,20 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
                     const int col = n * 128 + c * 64;
                     if (g.save) {
 #pragma unroll 1
-                        for (int part = 0; part < 2; ++part) {  // gate, up
+                        for (int part = 0; part < 4; ++part) {  // gate, up of 32 columns, gate, up of the next 32
+                            const int sub = (part & 1) * 128 + c * 64 + (part >> 1) * 32;
                             const uint32_t buf = next_buf();
+                            uint32_t p[32];
+                            tmem_ld_32x32b_x32(t_acc + sub, p);
+                            tmem_ld_wait(p);
 #pragma unroll
-                            for (int hi = 0; hi < 2; ++hi) {
-                                float f[32];
-                                uint32_t p[16];
-                                ld_acc(t_acc + part * 128 + c * 64 + hi * 32, f);
-                                pack32(f, p);
-                                stage_half(buf, lane, hi, p);
+                            for (int j = 0; j < 8; ++j) {
+                                const uint32_t addr = buf + lane * 128 + ((j ^ (lane & 7)) << 4);
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(p[4 * j]),
+                                             "r"(p[4 * j + 1]), "r"(p[4 * j + 2]), "r"(p[4 * j + 3])
+                                             : "memory");
                             }
-                            send(buf, &maps.out[1 + part], col, row0);
+                            send(buf, &maps.out[1 + (part & 1)], col + (part >> 1) * 32, row0, 2);
                         }
                     }
                     const uint32_t buf = next_buf();
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
             } else {
                 const int row = row0 + lane;
                 const bool row_ok = row < g.M;
-                const __nv_bfloat16* gu = g.gu + static_cast<size_t>(row) * (2 * static_cast<size_t>(g.N));
+                const float* gu = g.gu + static_cast<size_t>(row) * (2 * static_cast<size_t>(g.N));
 #pragma unroll 1
                 for (int c = 0; c < BN / 64; ++c) {
                     const int col0 = n * BN + c * 64;
@@ -407,16 +410,20 @@ static int product(const void* A, const void* B, void* D, int M, int N, int K, v
     if (rc != DK_OK) return rc;
     rc = operand_map(&maps.b, B, B_MN, EPI == EPI_GATED ? 2 * N : N, K, EPI == EPI_GATED ? 128 : BN);
     if (rc != DK_OK) return rc;
-    const uint64_t wide = static_cast<uint64_t>(N) * 4;  // bytes of a [g|u] row
-    auto out = [&](int i, void* p, uint64_t stride) { return make_tmap_2d(&maps.out[i], p, 2, N, M, stride, 64, 32); };
-    char* const pair = static_cast<char*>(EPI == EPI_DGATED ? D : gu);
+    // a map counts bf16 units: `words` of them to an element
+    auto out = [&](int i, void* p, uint64_t stride, int words) {
+        return make_tmap_2d(&maps.out[i], p, 2, static_cast<uint64_t>(N) * words, M, stride, 64, 32);
+    };
+    const uint64_t n = static_cast<uint64_t>(N);
     if (EPI == EPI_DGATED) {
-        rc = out(0, pair, wide);
-        if (rc == DK_OK) rc = out(1, pair + static_cast<size_t>(N) * 2, wide);
+        rc = out(0, D, 4 * n, 1);
+        if (rc == DK_OK) rc = out(1, static_cast<__nv_bfloat16*>(D) + n, 4 * n, 1);
     } else {
-        rc = out(0, D, static_cast<uint64_t>(N) * 2);
-        if (rc == DK_OK && EPI == EPI_GATED && gu != nullptr) rc = out(1, pair, wide);
-        if (rc == DK_OK && EPI == EPI_GATED && gu != nullptr) rc = out(2, pair + static_cast<size_t>(N) * 2, wide);
+        rc = out(0, D, 2 * n, 1);
+        if (EPI == EPI_GATED && gu != nullptr) {
+            if (rc == DK_OK) rc = out(1, gu, 8 * n, 2);
+            if (rc == DK_OK) rc = out(2, static_cast<float*>(gu) + n, 8 * n, 2);
+        }
     }
     if (rc != DK_OK) return rc;
     g.M = M;
@@ -426,7 +433,7 @@ static int product(const void* A, const void* B, void* D, int M, int N, int K, v
     g.tiles_n = (N + (EPI == EPI_GATED ? 128 : BN) - 1) / (EPI == EPI_GATED ? 128 : BN);
     g.group_m = 16;
     g.save = EPI == EPI_GATED && gu != nullptr;
-    g.gu = static_cast<const __nv_bfloat16*>(gu);
+    g.gu = static_cast<const float*>(gu);
     rc = device_status_ptr(&g.status);
     if (rc != DK_OK) return rc;
     return launch<A_MN, B_MN, EPI>(maps, g, st);
@@ -470,6 +477,7 @@ extern "C" int dk_gated_ffn_bwd(const void* dy, const void* x, const void* w13, 
         DK_CUDA_OK(cudaMemsetAsync(dw2, 0, static_cast<size_t>(F) * H * 2, st));
         return DK_OK;
     }
+    DK_REQUIRE((reinterpret_cast<uintptr_t>(gu) & 15) == 0, "gu must be 16-byte aligned");
     DK_REQUIRE(dy != nullptr && x != nullptr && gu != nullptr && h != nullptr && dgu != nullptr && dx != nullptr, "null operand");
     // dh = dy W2 (K = H, W2 [H,F] is [K,N]), straight into dg and du
     rc = product<false, true, EPI_DGATED>(dy, w2, dgu, T, F, H, const_cast<void*>(gu), st);

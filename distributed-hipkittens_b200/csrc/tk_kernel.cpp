@@ -618,7 +618,7 @@ py::object gated_ffn(py::object X, py::object W13, py::object W2, bool save) {
     PyObject* bf16 = a.x.dtype;
     void *gup = nullptr, *hp, *yp;
     py::object gu;
-    if (save) gu = new_empty(X, a.T, 2 * static_cast<int64_t>(a.F), bf16, &gup);
+    if (save) gu = new_empty(X, a.T, 2 * static_cast<int64_t>(a.F), torch_api().f32, &gup);
     py::object h = new_empty(X, a.T, a.F, bf16, &hp);
     py::object y = new_empty(X, a.T, a.H, bf16, &yp);
     throw_on(dk_gated_ffn(a.x.ptr, a.w13.ptr, a.w2.ptr, a.T, a.H, a.F, gup, hp, yp, stream_of(a.device)), "gated_ffn");
@@ -630,7 +630,7 @@ py::tuple gated_ffn_bwd(py::object dY, py::object X, py::object W13, py::object 
     const FfnArgs a = ffn_args(X, W13, W2);
     const Dense dy = dense_arg(dY, a.device, "dY"), gu = dense_arg(GU, a.device, "GU"), h = dense_arg(Hh, a.device, "H");
     want_dtype(dy, a.x.dtype, "dY", "torch.bfloat16");
-    want_dtype(gu, a.x.dtype, "GU", "torch.bfloat16");
+    want_dtype(gu, torch_api().f32, "GU", "torch.float32");
     want_dtype(h, a.x.dtype, "H", "torch.bfloat16");
     const int64_t F2 = 2 * static_cast<int64_t>(a.F);
     if (!dy.is(a.T, a.H) || !gu.is(a.T, F2) || !h.is(a.T, a.F))
@@ -706,7 +706,7 @@ PYBIND11_MODULE(tk_kernel, m) {
           "from the layers above) may be None");
     m.def("gated_ffn", &gated_ffn, py::arg("X"), py::arg("W13"), py::arg("W2"), py::arg("save") = false,
           "Y = (silu(X Wg^T) * (X Wu^T)) W2^T, bf16: X [T,H], W13 [2F,H] (gate rows, then up rows), W2 [H,F]. "
-          "save: (Y, GU [T,2F], H [T,F]) for gated_ffn_bwd");
+          "save: (Y, GU fp32 [T,2F], H [T,F]) for gated_ffn_bwd");
     m.def("gated_ffn_bwd", &gated_ffn_bwd, py::arg("dY"), py::arg("X"), py::arg("W13"), py::arg("W2"), py::arg("GU"),
           py::arg("H"), "(dX, dW13, dW2) of gated_ffn, from what it saved");
     m.def("device_status", &device_status,

@@ -278,7 +278,7 @@ def gated_ffn_train(x: torch.Tensor, w13: torch.Tensor,
 def _(x, w13, w2):
     _ffn_shapes(x, w13, w2)
     T, F = x.shape[0], w2.shape[1]
-    return torch.empty_like(x), x.new_empty((T, 2 * F)), x.new_empty((T, F))
+    return torch.empty_like(x), x.new_empty((T, 2 * F), dtype=torch.float32), x.new_empty((T, F))
 
 
 @torch.library.custom_op(f"{NS}::gated_ffn_bwd", mutates_args=(), device_types="cuda")

@@ -515,13 +515,13 @@ int dk_add_rms_norm_bwd(const void* dy, const void* dr, const void* r, const flo
 /* ------------------------------------------------------------------ gated feed-forward block, bf16 */
 /*
  * No counterpart in the reference's distributed path. x [T, H], w13 [2F, H] (F gate rows, then F up rows, the
- * layout of the MoE entry points), w2 [H, F], all bf16, rows contiguous; H and F multiples of 8.
+ * layout of the MoE entry points), w2 [H, F], all bf16, rows contiguous, 16-byte aligned; H and F multiples of 8.
  *   [g | u] = x w13^T;  h = silu(g) * u  [T, F];  y = h w2^T  [T, H]
  * dk_gated_ffn: both projections, the activation and the product in one kernel, then the down projection. h is
- * an output and the second kernel's input; gu [T, 2F] (g, then u in every row) is written when it is not
- * NULL. fp32 accumulation; g and u enter silu(g) * u in fp32, h, g, u and y are rounded to bf16 once. T == 0
+ * an output and the second kernel's input; gu [T, 2F] fp32 (g, then u in every row) is written when it is not
+ * NULL. fp32 accumulation; g and u enter silu(g) * u in fp32, h and y are rounded to bf16 once. T == 0
  * launches nothing.
- * dk_gated_ffn_bwd: from dy and the kept gu and h: dx [T, H], dw13 [2F, H], dw2 [H, F]; dgu [T, 2F] is
+ * dk_gated_ffn_bwd: from dy and the kept gu and h: dx [T, H], dw13 [2F, H], dw2 [H, F]; dgu [T, 2F] bf16 is
  * workspace (the gradient of gu afterwards). T == 0 clears the weight gradients.
  * One rank of a tensor-parallel block: w13 and w2 hold its F / P inner columns, y (and dx) are then summed over
  * the ranks with dk_allreduce.
