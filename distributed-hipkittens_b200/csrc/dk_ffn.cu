@@ -21,10 +21,16 @@
 // their roundings entered too (0.0030). The price is 8 bytes a value of h instead of 4, written and read beside
 // matrix products.
 //
-//   warp 0      TMA producer: 128-byte-swizzled boxes into a four-stage ring
-//   warp 1      one thread issues tcgen05.mma 128x256x16 into one of two 256-column accumulators
+//   warp 0      TMA producer: 128-byte-swizzled boxes into a ring of stages
+//   warp 1      one thread issues tcgen05.mma into one of two 256-column accumulators
 //   warps 2-5   epilogue: tcgen05.ld, swizzled staging in shared memory, TMA stores (which clip the
 //               ragged edges)
+//
+// PAIR = 2: a cluster of two CTAs per 256x256 tile (cta_group::2). Each stages its 128 rows of A and half of
+// the B tile (gated: CTA 0 the gate rows, CTA 1 the up rows), so a stage is 32 KiB instead of 48, the ring six
+// deep instead of four, and a flop needs two thirds of the shared-memory fill. Both CTAs' loads complete on the
+// leader's barrier, the leader issues the MMAs. PAIR = 1: one CTA per 128x256 tile, for row counts whose last pair
+// would be half empty.
 #include "dk_host.h"
 #include "dk_ptx.cuh"
 
@@ -37,13 +43,17 @@ constexpr int BN = 256;
 constexpr int BK = 64;  // 64 bf16 = 128 bytes = one swizzle row
 constexpr int UMMA_K = 16;
 constexpr int A_BYTES = BM * BK * 2;
-constexpr int B_BYTES = BN * BK * 2;
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int STAGES = 4;
 constexpr int MN_BLOCK = 64 * BK * 2;  // an MN-major box: 64 elements of M or N (128 bytes) x 64 of K
 constexpr int EPI_BUF = 32 * 128;      // 32 rows x 64 bf16
 constexpr int EPI_BYTES = 4 * 2 * EPI_BUF;
-constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + 256;
+template <int PAIR>
+struct Cfg {
+    static constexpr int B_ROWS = BN / PAIR;
+    static constexpr int B_BYTES = B_ROWS * BK * 2;
+    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = PAIR == 2 ? 6 : 4;
+    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + 256;
+};
 constexpr int THREADS = 192;
 constexpr int TMEM_COLS = 512;
 
@@ -57,7 +67,7 @@ struct Maps {
 
 struct Args {
     int M, N, num_kb;  // N: columns of the output (GATED, DGATED: F)
-    int tiles_m, tiles_n, group_m;
+    int tiles_m, tiles_n, group_m;  // tiles of 128 * PAIR rows
     int save;                 // GATED: g and u leave too
     const float* gu;          // DGATED: kept [g|u], [M, 2N]
     unsigned* status;
@@ -124,8 +134,9 @@ __device__ __forceinline__ void ld_row32(const float* p, int col, int n, bool ok
     }
 }
 
-template <bool A_MN, bool B_MN, int EPI>
+template <bool A_MN, bool B_MN, int EPI, int PAIR>
 __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_constant__ Maps maps, const Args g) {
+    constexpr int STAGES = Cfg<PAIR>::STAGES, STAGE_BYTES = Cfg<PAIR>::STAGE_BYTES, B_ROWS = Cfg<PAIR>::B_ROWS;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t ring = smem_base;
@@ -139,6 +150,8 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtx wc{g.status, abort_sm};
+    const int crank = PAIR == 2 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int unit = blockIdx.x / PAIR, nunits = gridDim.x / PAIR;
     const int num_tiles = g.tiles_m * g.tiles_n;
 
     if (threadIdx.x == 0) {
@@ -149,18 +162,23 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(bar_tfull + 8 * a, 1);
-            mbar_init(bar_tempty + 8 * a, 128);
+            mbar_init(bar_tempty + 8 * a, 128 * PAIR);  // the leader hears both CTAs' epilogues
         }
         fence_mbar_init();
         tma_prefetch_desc(&maps.a);
         tma_prefetch_desc(&maps.b);
     }
     if (warp == 1) {
-        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
-        tmem_relinquish<1>();
+        tmem_alloc<PAIR>(smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
+        tmem_relinquish<PAIR>();
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR == 2) {
+        // both CTAs' barriers exist before either signals the other's
+        cluster_arrive();
+        cluster_wait();
+    }
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
@@ -169,31 +187,41 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
             int s = 0;
             uint32_t ph = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+            for (int t = unit; t < num_tiles && ok; t += nunits) {
                 int m, n;
                 tile_coords(t, g, m, n);
+                m = m * PAIR + crank;  // this CTA's 128-row tile
                 for (int kb = 0; kb < g.num_kb; ++kb) {
                     if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, wc, SITE_EMPTY, t)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t full = bar_full + 8 * s, sa = ring + s * STAGE_BYTES, sb = sa + A_BYTES;
-                    mbar_expect_tx(full, STAGE_BYTES);
+                    const uint32_t sa = ring + s * STAGE_BYTES, sb = sa + A_BYTES;
+                    // a pair's loads complete on the leader's barrier, which expects the bytes of both CTAs
+                    const uint32_t full = PAIR == 2 ? mapa_shared(bar_full + 8 * s, 0) : bar_full + 8 * s;
+                    if (crank == 0) mbar_expect_tx(bar_full + 8 * s, PAIR * STAGE_BYTES);
+                    auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+                        if (PAIR == 2) tma_load_2d_pair(dst, map, full, x, y);
+                        else tma_load_2d(dst, map, full, x, y);
+                    };
                     if (A_MN) {
-                        for (int i = 0; i < BM / 64; ++i)
-                            tma_load_2d(sa + i * MN_BLOCK, &maps.a, full, m * BM + 64 * i, kb * BK);
+                        for (int i = 0; i < BM / 64; ++i) load(sa + i * MN_BLOCK, &maps.a, m * BM + 64 * i, kb * BK);
                     } else {
-                        tma_load_2d(sa, &maps.a, full, kb * BK, m * BM);
+                        load(sa, &maps.a, kb * BK, m * BM);
                     }
                     if (EPI == EPI_GATED) {
                         // gate rows that do not exist read up rows instead, up rows zeros: not stored
-                        tma_load_2d(sb, &maps.b, full, kb * BK, n * 128);
-                        tma_load_2d(sb + B_BYTES / 2, &maps.b, full, kb * BK, g.N + n * 128);
+                        if (PAIR == 2) {
+                            load(sb, &maps.b, kb * BK, crank * g.N + n * 128);
+                        } else {
+                            load(sb, &maps.b, kb * BK, n * 128);
+                            load(sb + 128 * BK * 2, &maps.b, kb * BK, g.N + n * 128);
+                        }
                     } else if (B_MN) {
-                        for (int i = 0; i < BN / 64; ++i)
-                            tma_load_2d(sb + i * MN_BLOCK, &maps.b, full, n * BN + 64 * i, kb * BK);
+                        for (int i = 0; i < B_ROWS / 64; ++i)
+                            load(sb + i * MN_BLOCK, &maps.b, n * BN + crank * B_ROWS + 64 * i, kb * BK);
                     } else {
-                        tma_load_2d(sb, &maps.b, full, kb * BK, n * BN);
+                        load(sb, &maps.b, kb * BK, n * BN + crank * B_ROWS);
                     }
                     if (++s == STAGES) {
                         s = 0;
@@ -203,15 +231,15 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = umma_idesc(1, 1, BM, BN) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+        if (lane == 0 && crank == 0) {
+            constexpr uint32_t idesc = umma_idesc(1, 1, BM * PAIR, BN) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
             // descriptor steps of 16 elements of K, in 16-byte units: 32 bytes along the swizzle row, or
             // 16 rows of 128 bytes
             constexpr uint64_t a_step = A_MN ? 16 * 128 / 16 : 2, b_step = B_MN ? 16 * 128 / 16 : 2;
             int s = 0, acc = 0;
             uint32_t ph = 0, acc_ph = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+            for (int t = unit; t < num_tiles && ok; t += nunits) {
                 if (!mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, wc, SITE_TMEM_EMPTY, t)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * BN;
@@ -226,15 +254,18 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
                     const uint64_t db = B_MN ? desc_mn(sb) : umma_desc_sw128(sb);
 #pragma unroll
                     for (int k = 0; k < BK / UMMA_K; ++k)
-                        umma_f16<1>(d_tmem, da + a_step * k, db + b_step * k, idesc, (kb | k) != 0);
-                    umma_commit<1>(bar_empty + 8 * s);
+                        umma_f16<PAIR>(d_tmem, da + a_step * k, db + b_step * k, idesc, (kb | k) != 0);
+                    // the stage is free in both CTAs once these MMAs have read it
+                    if (PAIR == 2) umma_commit_pair(bar_empty + 8 * s, 3);
+                    else umma_commit<1>(bar_empty + 8 * s);
                     if (++s == STAGES) {
                         s = 0;
                         ph ^= 1;
                     }
                 }
                 if (!ok) break;
-                umma_commit<1>(bar_tfull + 8 * acc);
+                if (PAIR == 2) umma_commit_pair(bar_tfull + 8 * acc, 3);
+                else umma_commit<1>(bar_tfull + 8 * acc);
                 acc ^= 1;
                 if (acc == 0) acc_ph ^= 1;
             }
@@ -259,10 +290,10 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
                 tma_store_commit();
             }
         };
-        for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+        for (int t = unit; t < num_tiles; t += nunits) {
             int m, n;
             tile_coords(t, g, m, n);
-            const int row0 = m * BM + q * 32;
+            const int row0 = (m * PAIR + crank) * BM + q * 32;
             if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, acc_ph, wc, SITE_TMEM_FULL, t))) break;
             tc_fence_after();
             const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
@@ -352,7 +383,8 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
                 }
             }
             tc_fence_before();
-            mbar_arrive(bar_tempty + 8 * acc);
+            if (PAIR == 2 && crank != 0) mbar_arrive_cluster(mapa_shared(bar_tempty + 8 * acc, 0));
+            else mbar_arrive(bar_tempty + 8 * acc);
             acc ^= 1;
             if (acc == 0) acc_ph ^= 1;
         }
@@ -361,6 +393,11 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
 
     tc_fence_before();
     __syncthreads();
+    if (PAIR == 2) {
+        // neither CTA leaves (or frees the pair's TMEM) while the other may still signal it
+        cluster_arrive();
+        cluster_wait();
+    }
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
@@ -370,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
             while (globaltimer_ns() - t0 < 200000ull) {
             }
         }
-        tmem_dealloc<1>(tmem_base, TMEM_COLS);
+        tmem_dealloc<PAIR>(tmem_base, TMEM_COLS);
     }
 }
 
@@ -383,22 +420,40 @@ static int operand_map(CUtensorMap* map, const void* p, bool mn, int rows_or_col
     return make_tmap_2d(map, p, 2, K, rows_or_cols, static_cast<uint64_t>(K) * 2, BK, box);
 }
 
-template <bool A_MN, bool B_MN, int EPI>
+template <bool A_MN, bool B_MN, int EPI, int PAIR>
 static int launch(const Maps& maps, const Args& g, cudaStream_t st) {
+    const auto kernel = ffn_gemm_kernel<A_MN, B_MN, EPI, PAIR>;
     static bool attr_set[64] = {false};
     int dev = 0, sms = 0;
     DK_CUDA_OK(cudaGetDevice(&dev));
     if (!attr_set[dev & 63]) {
-        DK_CUDA_OK(cudaFuncSetAttribute(ffn_gemm_kernel<A_MN, B_MN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        SMEM_BYTES));
+        DK_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<PAIR>::SMEM_BYTES));
         attr_set[dev & 63] = true;
     }
     const int rc = sm_count(&sms);
     if (rc != DK_OK) return rc;
     const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
-    ffn_gemm_kernel<A_MN, B_MN, EPI><<<static_cast<int>(tiles < sms ? tiles : sms), THREADS, SMEM_BYTES, st>>>(maps, g);
-    DK_CUDA_OK(cudaGetLastError());
+    const int units = sms / PAIR;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<int>(tiles < units ? tiles : units) * PAIR);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Cfg<PAIR>::SMEM_BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = PAIR;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    DK_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, maps, g));
     return DK_OK;
+}
+
+// Two-CTA tiles unless more than one row tile in nine would be computed for nothing.
+static bool use_pair(int M) {
+    const int tiles = (M + BM - 1) / BM;
+    return tiles % 2 == 0 || tiles >= 9;
 }
 
 // D[M,N] = A B. GATED: B = W13 [2N, K], D = h. DGATED: D = dgu [M, 2N].
@@ -406,9 +461,10 @@ template <bool A_MN, bool B_MN, int EPI>
 static int product(const void* A, const void* B, void* D, int M, int N, int K, void* gu, cudaStream_t st) {
     Maps maps;
     Args g{};
+    const int pair = use_pair(M) ? 2 : 1;
     int rc = operand_map(&maps.a, A, A_MN, M, K, BM);
     if (rc != DK_OK) return rc;
-    rc = operand_map(&maps.b, B, B_MN, EPI == EPI_GATED ? 2 * N : N, K, EPI == EPI_GATED ? 128 : BN);
+    rc = operand_map(&maps.b, B, B_MN, EPI == EPI_GATED ? 2 * N : N, K, EPI == EPI_GATED ? 128 : BN / pair);
     if (rc != DK_OK) return rc;
     // a map counts bf16 units: `words` of them to an element
     auto out = [&](int i, void* p, uint64_t stride, int words) {
@@ -429,14 +485,14 @@ static int product(const void* A, const void* B, void* D, int M, int N, int K, v
     g.M = M;
     g.N = N;
     g.num_kb = (K + BK - 1) / BK;
-    g.tiles_m = (M + BM - 1) / BM;
+    g.tiles_m = (M + BM * pair - 1) / (BM * pair);
     g.tiles_n = (N + (EPI == EPI_GATED ? 128 : BN) - 1) / (EPI == EPI_GATED ? 128 : BN);
-    g.group_m = 16;
+    g.group_m = 16 / pair;
     g.save = EPI == EPI_GATED && gu != nullptr;
     g.gu = static_cast<const float*>(gu);
     rc = device_status_ptr(&g.status);
     if (rc != DK_OK) return rc;
-    return launch<A_MN, B_MN, EPI>(maps, g, st);
+    return pair == 2 ? launch<A_MN, B_MN, EPI, 2>(maps, g, st) : launch<A_MN, B_MN, EPI, 1>(maps, g, st);
 }
 
 static int check_shape(int T, int H, int F) {
