@@ -412,6 +412,217 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
 }
 
 // --------------------------------------------------------------------------------------------
+// Few rows (single tokens, batches of sequences being answered): bound by reading the weights once. The roles are
+// swapped: 128 weight rows are the tensor core's M, the tokens its N (padded to 16..256), so a tile is 16 KB of
+// weights per 64 of K whatever the number of tokens, and F / 64 or H / 128 tiles are cut along K over a cluster
+// of S CTAs until there are enough CTAs to draw on all of HBM. Each CTA leaves its fp32 partial sums in its own
+// shared memory; the cluster's CTAs then add up each other's through distributed shared memory, in rank order: no
+// workspace, no second launch, the same bits on every run.
+//   GATED: a tile is 64 gate rows and the 64 up rows of the same columns; silu(g) * u leaves.
+// The second product (from h) may start while the first still runs: its weights do not depend on the first, so the
+// ring is filled with them, and only then does it wait for the rows of h.
+constexpr int ROWS_THREADS = 192;
+template <int N>
+struct RowsCfg {
+    static constexpr int W_BYTES = 128 * BK * 2;
+    static constexpr int STAGE = W_BYTES + N * BK * 2;
+    // two CTAs per SM up to 128 tokens, one for 256
+    static constexpr int STAGES = N <= 32 ? 5 : N == 64 ? 4 : N == 128 ? 3 : 4;
+    static constexpr int CTAS_PER_SM = N <= 128 ? 2 : 1;
+    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE + 128;
+    static constexpr int TMEM = N < 32 ? 32 : N;
+    static_assert(N * 128 * 4 <= STAGES * STAGE, "the partial sums reuse the ring");
+};
+struct RowsMaps {
+    CUtensorMap w, x;
+};
+struct RowsArgs {
+    int T, cols, num_kb;  // cols: columns of the output (F or H)
+    __nv_bfloat16* out;   // [T, cols]
+    float* gu;            // GATED: [T, 2 cols], may be null
+    unsigned* status;
+};
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+template <bool GATED, int N>
+__global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsArgs g) {
+    using C = RowsCfg<N>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t ctrl = ring + C::STAGES * C::STAGE;
+    uint8_t* ctrl_p = smem_raw + (ctrl - smem_u32(smem_raw));
+    const uint32_t bar_full = ctrl, bar_empty = ctrl + 8 * C::STAGES, bar_done = ctrl + 16 * C::STAGES;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl_p + 16 * C::STAGES + 8);
+    volatile int* abort_sm = reinterpret_cast<volatile int*>(ctrl_p + 16 * C::STAGES + 16);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const WaitCtx wc{g.status, abort_sm};
+    uint32_t split;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(split));
+    const int S = static_cast<int>(split), rank = static_cast<int>(cluster_ctarank());
+    const int tile = blockIdx.x / S;
+    const int tok0 = blockIdx.y * N;
+    const int kb0 = static_cast<int>(static_cast<int64_t>(rank) * g.num_kb / S);
+    const int kb1 = static_cast<int>(static_cast<int64_t>(rank + 1) * g.num_kb / S);
+
+    if (threadIdx.x == 0) {
+        *abort_sm = 0;
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        mbar_init(bar_done, 1);
+        fence_mbar_init();
+        tma_prefetch_desc(&maps.w);
+        tma_prefetch_desc(&maps.x);
+    }
+    if (warp == 1) {
+        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), C::TMEM);
+        tmem_relinquish<1>();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // the next kernel's CTAs may take the places that this one's leave
+    if (GATED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (warp == 0) {
+        if (lane == 0) {
+            auto load_w = [&](int kb, int s) {
+                const uint32_t sw = ring + s * C::STAGE, full = bar_full + 8 * s;
+                mbar_expect_tx(full, C::STAGE);
+                if (GATED) {
+                    // gate rows that do not exist read up rows instead, up rows zeros: not stored
+                    tma_load_2d(sw, &maps.w, full, kb * BK, tile * 64);
+                    tma_load_2d(sw + C::W_BYTES / 2, &maps.w, full, kb * BK, g.cols + tile * 64);
+                } else {
+                    tma_load_2d(sw, &maps.w, full, kb * BK, tile * 128);
+                }
+            };
+            auto load_x = [&](int kb, int s) {
+                tma_load_2d(ring + s * C::STAGE + C::W_BYTES, &maps.x, bar_full + 8 * s, kb * BK, tok0);
+            };
+            const int ahead = min(kb1 - kb0, C::STAGES);
+            for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
+            if (!GATED) {
+                // h is complete and visible from here on, to the copy engine too
+                asm volatile("griddepcontrol.wait;" ::: "memory");
+                asm volatile("fence.proxy.async;" ::: "memory");
+            }
+            for (int i = 0; i < ahead; ++i) load_x(kb0 + i, i);
+            int s = 0;
+            uint32_t ph = 0;
+            for (int kb = kb0 + ahead; kb < kb1; ++kb) {
+                if (!mbar_wait(bar_empty + 8 * s, ph, wc, SITE_EMPTY, tile)) break;
+                load_w(kb, s);
+                load_x(kb, s);
+                if (++s == C::STAGES) {
+                    s = 0;
+                    ph ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = umma_idesc(1, 1, 128, N);
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(bar_full + 8 * s, ph, wc, SITE_FULL, tile)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint64_t da = umma_desc_sw128(ring + s * C::STAGE);
+                const uint64_t db = umma_desc_sw128(ring + s * C::STAGE + C::W_BYTES);
+#pragma unroll
+                for (int k = 0; k < BK / UMMA_K; ++k) umma_f16<1>(tmem, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
+                umma_commit<1>(bar_empty + 8 * s);
+                if (++s == C::STAGES) {
+                    s = 0;
+                    ph ^= 1;
+                }
+            }
+            if (ok) umma_commit<1>(bar_done);
+        }
+    } else {
+        // partial sums as [token][weight row]; every load has been consumed, so the ring is free
+        const int q = warp & 3;
+        if (__all_sync(0xffffffffu, mbar_wait(bar_done, 0, wc, SITE_TMEM_FULL, tile))) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < N; c += 32) {
+                if (tok0 + c >= g.T) break;
+                uint32_t r[32];
+                tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, r);
+                tmem_ld_wait(r);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c + j < N)
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring + ((c + j) * 128 + q * 32 + lane) * 4), "r"(r[j])
+                                     : "memory");
+            }
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    {
+        constexpr int PAIRS = GATED ? 32 : 64;  // pairs of neighbouring output columns of a tile
+        const int count = min(N, g.T - tok0) * PAIRS;
+        for (int e = rank * ROWS_THREADS + threadIdx.x; e < count; e += S * ROWS_THREADS) {
+            const int n = e / PAIRS, p = e % PAIRS;
+            const int col = tile * (2 * PAIRS) + 2 * p;
+            const uint32_t at = ring + (n * 128 + 2 * p) * 4;
+            float2 a = make_float2(0.f, 0.f), b = make_float2(0.f, 0.f);
+            for (int s = 0; s < S; ++s) {
+                const uint32_t peer = mapa_shared(at, s);
+                const float2 v = ld_cluster_f2(peer);
+                a.x += v.x;
+                a.y += v.y;
+                if (GATED) {
+                    const float2 u = ld_cluster_f2(peer + 64 * 4);
+                    b.x += u.x;
+                    b.y += u.y;
+                }
+            }
+            if (col >= g.cols) continue;
+            const size_t row = static_cast<size_t>(tok0 + n);
+            if (GATED) {
+                if (g.gu != nullptr) {
+                    float* gu = g.gu + row * (2 * static_cast<size_t>(g.cols)) + col;
+                    *reinterpret_cast<float2*>(gu) = a;
+                    *reinterpret_cast<float2*>(gu + g.cols) = b;
+                }
+                a.x = a.x * sigmoid_f(a.x) * b.x;
+                a.y = a.y * sigmoid_f(a.y) * b.y;
+            }
+            *reinterpret_cast<uint32_t*>(g.out + row * g.cols + col) = pack_bf16x2(a.x, a.y);
+        }
+    }
+    // a CTA's partial sums stay until every peer has read them
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (warp == 1) {
+        tc_fence_after();
+        if (*abort_sm) {
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 200000ull) {
+            }
+        }
+        tmem_dealloc<1>(tmem, C::TMEM);
+    }
+}
+
+// --------------------------------------------------------------------------------------------
 // host side
 
 // K-major operand [rows, K] or MN-major operand [K, cols]; `box` rows of a K-major one
@@ -495,6 +706,72 @@ static int product(const void* A, const void* B, void* D, int M, int N, int K, v
     return pair == 2 ? launch<A_MN, B_MN, EPI, 2>(maps, g, st) : launch<A_MN, B_MN, EPI, 1>(maps, g, st);
 }
 
+template <bool GATED, int N>
+static int launch_rows(const RowsMaps& maps, const RowsArgs& g, int tiles, int S, cudaStream_t st) {
+    using C = RowsCfg<N>;
+    const auto kernel = ffn_rows_kernel<GATED, N>;
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    DK_CUDA_OK(cudaGetDevice(&dev));
+    if (!attr_set[dev & 63]) {
+        DK_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+        attr_set[dev & 63] = true;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(tiles * S, (g.T + N - 1) / N);
+    cfg.blockDim = dim3(ROWS_THREADS);
+    cfg.dynamicSmemBytes = C::SMEM_BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    // the second product overlaps the end of the first, which is the kernel before it on the stream
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = GATED ? 1 : 2;
+    DK_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, maps, g));
+    return DK_OK;
+}
+
+// out [T, cols] = x W^T for few rows; GATED: W = W13, out = h
+template <bool GATED>
+static int rows_product(const void* x, const void* W, void* out, int T, int cols, int K, void* gu, cudaStream_t st) {
+    int sms = 0;
+    int rc = sm_count(&sms);
+    if (rc != DK_OK) return rc;
+    const int N = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+    RowsMaps maps;
+    rc = make_tmap_2d(&maps.w, W, 2, K, GATED ? 2 * cols : cols, static_cast<uint64_t>(K) * 2, BK, GATED ? 64 : 128);
+    if (rc == DK_OK) rc = make_tmap_2d(&maps.x, x, 2, K, T, static_cast<uint64_t>(K) * 2, BK, N);
+    if (rc != DK_OK) return rc;
+    RowsArgs g{};
+    g.T = T;
+    g.cols = cols;
+    g.num_kb = (K + BK - 1) / BK;
+    g.out = static_cast<__nv_bfloat16*>(out);
+    g.gu = static_cast<float*>(gu);
+    rc = device_status_ptr(&g.status);
+    if (rc != DK_OK) return rc;
+    const int tiles = (cols + (GATED ? 64 : 128) - 1) / (GATED ? 64 : 128);
+    // cut K while the CTAs still run all at once and each keeps a few K blocks
+    const int places = sms * (N <= 128 ? 2 : 1);
+    int S = 1;
+    while (S < 8 && tiles * S * 2 * ((T + N - 1) / N) <= places && g.num_kb / (S * 2) >= 4) S *= 2;
+    switch (N) {
+        case 16: return launch_rows<GATED, 16>(maps, g, tiles, S, st);
+        case 32: return launch_rows<GATED, 32>(maps, g, tiles, S, st);
+        case 64: return launch_rows<GATED, 64>(maps, g, tiles, S, st);
+        case 128: return launch_rows<GATED, 128>(maps, g, tiles, S, st);
+        default: return launch_rows<GATED, 256>(maps, g, tiles, S, st);
+    }
+}
+
+// Few rows: see ffn_rows_kernel.
+constexpr int ROWS_MAX_T = 256;
+
 static int check_shape(int T, int H, int F) {
     DK_REQUIRE(T >= 0, "the number of rows must not be negative");
     DK_REQUIRE(H >= 8 && F >= 8 && H % 8 == 0 && F % 8 == 0, "H and F must be positive multiples of 8");
@@ -515,6 +792,13 @@ extern "C" int dk_gated_ffn(const void* x, const void* w13, const void* w2, int 
     if (T == 0) return DK_OK;
     DK_REQUIRE(x != nullptr && h != nullptr && y != nullptr, "null operand");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    DK_REQUIRE(((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(gu)) & 15) == 0,
+               "h, y and gu must be 16-byte aligned");
+    if (T <= ROWS_MAX_T) {
+        rc = rows_product<true>(x, w13, h, T, F, H, gu, st);
+        if (rc != DK_OK) return rc;
+        return rows_product<false>(h, w2, y, T, H, F, nullptr, st);
+    }
     rc = product<false, false, EPI_GATED>(x, w13, h, T, F, H, gu, st);
     if (rc != DK_OK) return rc;
     return product<false, false, EPI_STORE>(h, w2, y, T, H, F, nullptr, st);
