@@ -7,15 +7,16 @@
 //   dh = dy W2,  dg = dh * u * s * (1 + g * (1 - s)),  du = dh * g * s
 //   dx = [dg|du] W13,  dW13 = [dg|du]^T x,  dW2 = dy^T h
 //
-// One kernel serves all six products, D[M,N] = A B with fp32 accumulation in tensor memory. It is
-// instantiated over how the operands lie in memory: K-major ([M,K] and [N,K], the weights of a
-// forward pass) or MN-major ([K,M] and [K,N]: W2 and W13 seen from the other side, and the token axis as
-// K in the weight gradients), which the tensor core reads through a descriptor of its own, so nothing is
-// transposed in memory. What it does with a finished tile:
+// One kernel serves all six products, D[M,N] = A B with fp32 accumulation in tensor memory. Its operands lie in
+// memory K-major ([M,K] and [N,K], the weights of a forward pass) or MN-major ([K,M] and [K,N]: W2 and W13 seen from
+// the other side, and the token axis as K in the weight gradients), which the tensor core reads through a
+// descriptor of its own, so nothing is transposed in memory. What it does with a finished tile:
 //   EPI_STORE   bf16 rows of D
-//   EPI_GATED   the B tile is 128 gate rows and 128 up rows, so a thread holds g and u of the same
+//   EPI_GATED   the B tile is as many gate rows as up rows, so a thread holds g and u of the same
 //               place: silu(g) * u leaves as h, and g, u too when a backward pass will follow
 //   EPI_DGATED  D is dh: with the kept g, u of the same place, dg and du leave
+// A launch takes up to three products of one kind, their tiles in one list: dx, dW13 and dW2 need no launch of their
+// own, and the last wave of one is filled by the next.
 // h, dg and du are rounded to bf16, the type in which the tensor core takes them up again. g and u are kept in
 // 32 bits: dx and dW13 then carry two roundings, [dg|du] and their own (error against 64 bits 0.0024); kept in bf16
 // their roundings entered too (0.0030). The price is 8 bytes a value of h instead of 4, written and read beside
@@ -34,42 +35,47 @@
 #include "dk_host.h"
 #include "dk_ptx.cuh"
 
+#include <initializer_list>
+
 namespace dk {
 
 namespace ffn {
 
 constexpr int BM = 128;
-constexpr int BN = 256;
+constexpr int BN_MAX = 256;  // a tile is 256, 192 or 128 columns wide, see choose()
 constexpr int BK = 64;  // 64 bf16 = 128 bytes = one swizzle row
 constexpr int UMMA_K = 16;
 constexpr int A_BYTES = BM * BK * 2;
 constexpr int MN_BLOCK = 64 * BK * 2;  // an MN-major box: 64 elements of M or N (128 bytes) x 64 of K
 constexpr int EPI_BUF = 32 * 128;      // 32 rows x 64 bf16
 constexpr int EPI_BYTES = 4 * 2 * EPI_BUF;
-template <int PAIR>
-struct Cfg {
-    static constexpr int B_ROWS = BN / PAIR;
-    static constexpr int B_BYTES = B_ROWS * BK * 2;
-    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = PAIR == 2 ? 6 : 4;
-    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + 256;
-};
+constexpr int RING_BYTES = 192 * 1024;  // as many stages as fit: 6 of 256 columns a pair, 8 of 128
+constexpr int MAX_STAGES = 8;
+constexpr int SMEM_BYTES = 1024 + RING_BYTES + EPI_BYTES + 256;
 constexpr int THREADS = 192;
 constexpr int TMEM_COLS = 512;
 
 enum : int { EPI_STORE = 0, EPI_GATED = 1, EPI_DGATED = 2 };
 enum : unsigned { SITE_EMPTY = 101, SITE_FULL = 102, SITE_TMEM_EMPTY = 103, SITE_TMEM_FULL = 104 };
 
+constexpr int MAX_PRODUCTS = 3;
 struct Maps {
-    CUtensorMap a, b;
-    CUtensorMap out[3];  // STORE: D; GATED: h, g, u; DGATED: dg, du
+    CUtensorMap a[MAX_PRODUCTS], b[MAX_PRODUCTS];
+    CUtensorMap out[MAX_PRODUCTS];  // STORE: D of each product; GATED: h, g, u; DGATED: dg, du
 };
 
-struct Args {
-    int M, N, num_kb;  // N: columns of the output (GATED, DGATED: F)
+struct Product {
+    int M, N, num_kb;               // N: columns of the output (GATED, DGATED: F)
     int tiles_m, tiles_n, group_m;  // tiles of 128 * PAIR rows
-    int save;                 // GATED: g and u leave too
-    const float* gu;          // DGATED: kept [g|u], [M, 2N]
+    int first;                      // the product's first tile in the launch's list
+    int a_mn, b_mn;
+};
+struct Args {
+    Product p[MAX_PRODUCTS];
+    int products, num_tiles;
+    int bn;           // width of the B tile (GATED: gate and up rows together)
+    int save;         // GATED: g and u leave too
+    const float* gu;  // DGATED: kept [g|u], [M, 2N]
     unsigned* status;
 };
 
@@ -86,19 +92,31 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t smem_addr) {
     return d;
 }
 
-// Column tiles run slowest inside a group of group_m row tiles, so that CTAs running together share
-// operand tiles in L2.
-__device__ __forceinline__ void tile_coords(int t, const Args& g, int& m, int& n) {
-    const int per_group = g.group_m * g.tiles_n;
+// Tile t of the list -> its product and place. Column tiles run slowest inside a group of group_m row tiles, so
+// that CTAs running together share operand tiles in L2.
+__device__ __forceinline__ int tile_coords(int t, const Args& g, int& m, int& n) {
+    int i = 0;
+    while (i + 1 < g.products && t >= g.p[i + 1].first) ++i;
+    const Product& p = g.p[i];
+    t -= p.first;
+    const int per_group = p.group_m * p.tiles_n;
     const int grp = t / per_group;
-    const int first = grp * g.group_m;
-    const int gsz = min(g.tiles_m - first, g.group_m);
+    const int first = grp * p.group_m;
+    const int gsz = min(p.tiles_m - first, p.group_m);
     const int r = t - grp * per_group;
     m = first + r % gsz;
     n = r / gsz;
+    return i;
 }
 
 __device__ __forceinline__ float sigmoid_f(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
+
+// dg, du of one value of h from dh and the kept g, u
+__device__ __forceinline__ void d_gated(float dh, float gate, float up, float& dg, float& du) {
+    const float s = sigmoid_f(gate);
+    du = dh * gate * s;
+    dg = dh * up * s * (1.0f + gate * (1.0f - s));
+}
 
 // 32 packed columns (64 bytes) of this lane's row into half `hi` of a swizzled 32x64 staging buffer.
 __device__ __forceinline__ void stage_half(uint32_t buf, int lane, int hi, const uint32_t (&p)[16]) {
@@ -134,29 +152,30 @@ __device__ __forceinline__ void ld_row32(const float* p, int col, int n, bool ok
     }
 }
 
-template <bool A_MN, bool B_MN, int EPI, int PAIR>
-__global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_constant__ Maps maps, const Args g) {
-    constexpr int STAGES = Cfg<PAIR>::STAGES, STAGE_BYTES = Cfg<PAIR>::STAGE_BYTES, B_ROWS = Cfg<PAIR>::B_ROWS;
+template <int EPI, int PAIR>
+__global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
+    const int bn = g.bn;
+    const int stage_bytes = A_BYTES + bn / PAIR * (BK * 2), stages = min(MAX_STAGES, RING_BYTES / stage_bytes);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t ring = smem_base;
-    const uint32_t epi = smem_base + STAGES * STAGE_BYTES;
+    const uint32_t epi = smem_base + RING_BYTES;
     const uint32_t ctrl = epi + EPI_BYTES;
     uint8_t* ctrl_p = smem_raw + (ctrl - smem_u32(smem_raw));
-    const uint32_t bar_full = ctrl, bar_empty = ctrl + 8 * STAGES;
-    const uint32_t bar_tfull = ctrl + 16 * STAGES, bar_tempty = bar_tfull + 16;
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl_p + 16 * STAGES + 32);
-    volatile int* abort_sm = reinterpret_cast<volatile int*>(ctrl_p + 16 * STAGES + 40);
+    const uint32_t bar_full = ctrl, bar_empty = ctrl + 8 * MAX_STAGES;
+    const uint32_t bar_tfull = ctrl + 16 * MAX_STAGES, bar_tempty = bar_tfull + 16;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl_p + 16 * MAX_STAGES + 32);
+    volatile int* abort_sm = reinterpret_cast<volatile int*>(ctrl_p + 16 * MAX_STAGES + 40);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtx wc{g.status, abort_sm};
     const int crank = PAIR == 2 ? static_cast<int>(cluster_ctarank()) : 0;
     const int unit = blockIdx.x / PAIR, nunits = gridDim.x / PAIR;
-    const int num_tiles = g.tiles_m * g.tiles_n;
+    const int num_tiles = g.num_tiles;
 
     if (threadIdx.x == 0) {
         *abort_sm = 0;
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(bar_full + 8 * s, 1);
             mbar_init(bar_empty + 8 * s, 1);
         }
@@ -165,8 +184,10 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
             mbar_init(bar_tempty + 8 * a, 128 * PAIR);  // the leader hears both CTAs' epilogues
         }
         fence_mbar_init();
-        tma_prefetch_desc(&maps.a);
-        tma_prefetch_desc(&maps.b);
+        for (int i = 0; i < g.products; ++i) {
+            tma_prefetch_desc(&maps.a[i]);
+            tma_prefetch_desc(&maps.b[i]);
+        }
     }
     if (warp == 1) {
         tmem_alloc<PAIR>(smem_u32(const_cast<uint32_t*>(tmem_slot)), TMEM_COLS);
@@ -181,91 +202,111 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
     }
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    // a kernel of the same call that follows may take the places this one's CTAs leave; this one, when it follows,
+    // reads nothing before the one before it is complete (everything else hangs on the producer's loads)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+    // Producer and issuer run their loops as whole warps and elect one thread for the instructions themselves: what
+    // the instructions take (descriptors, coordinates, barriers) then stays in uniform registers. With one thread
+    // in the loops a stage of 64 of K took 0.37 us to issue whatever its width; now 0.27 (128 columns).
     if (warp == 0) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int t = unit; t < num_tiles && ok; t += nunits) {
-                int m, n;
-                tile_coords(t, g, m, n);
-                m = m * PAIR + crank;  // this CTA's 128-row tile
-                for (int kb = 0; kb < g.num_kb; ++kb) {
-                    if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, wc, SITE_EMPTY, t)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t sa = ring + s * STAGE_BYTES, sb = sa + A_BYTES;
-                    // a pair's loads complete on the leader's barrier, which expects the bytes of both CTAs
-                    const uint32_t full = PAIR == 2 ? mapa_shared(bar_full + 8 * s, 0) : bar_full + 8 * s;
-                    if (crank == 0) mbar_expect_tx(bar_full + 8 * s, PAIR * STAGE_BYTES);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("fence.proxy.async;" ::: "memory");
+        const int b_rows = bn / PAIR;
+        const uint32_t tx = A_BYTES + b_rows * BK * 2;
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int t = unit; t < num_tiles && ok; t += nunits) {
+            int m, n;
+            const int pi = tile_coords(t, g, m, n);
+            const Product& p = g.p[pi];
+            m = m * PAIR + crank;  // this CTA's 128-row tile
+            for (int kb = 0; kb < p.num_kb; ++kb) {
+                if (!__all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, ph ^ 1, wc, SITE_EMPTY, t))) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t sa = ring + s * stage_bytes, sb = sa + A_BYTES;
+                // a pair's loads complete on the leader's barrier, which expects the bytes of both CTAs
+                const uint32_t full = PAIR == 2 ? mapa_shared(bar_full + 8 * s, 0) : bar_full + 8 * s;
+                if (elect_one()) {
+                    if (crank == 0) mbar_expect_tx(bar_full + 8 * s, PAIR * tx);
                     auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
                         if (PAIR == 2) tma_load_2d_pair(dst, map, full, x, y);
                         else tma_load_2d(dst, map, full, x, y);
                     };
-                    if (A_MN) {
-                        for (int i = 0; i < BM / 64; ++i) load(sa + i * MN_BLOCK, &maps.a, m * BM + 64 * i, kb * BK);
+                    if (p.a_mn) {
+                        for (int i = 0; i < BM / 64; ++i) load(sa + i * MN_BLOCK, &maps.a[pi], m * BM + 64 * i, kb * BK);
                     } else {
-                        load(sa, &maps.a, kb * BK, m * BM);
+                        load(sa, &maps.a[pi], kb * BK, m * BM);
                     }
                     if (EPI == EPI_GATED) {
                         // gate rows that do not exist read up rows instead, up rows zeros: not stored
+                        const int half = bn / 2;
                         if (PAIR == 2) {
-                            load(sb, &maps.b, kb * BK, crank * g.N + n * 128);
+                            load(sb, &maps.b[0], kb * BK, crank * p.N + n * half);
                         } else {
-                            load(sb, &maps.b, kb * BK, n * 128);
-                            load(sb + 128 * BK * 2, &maps.b, kb * BK, g.N + n * 128);
+                            load(sb, &maps.b[0], kb * BK, n * half);
+                            load(sb + half * BK * 2, &maps.b[0], kb * BK, p.N + n * half);
                         }
-                    } else if (B_MN) {
-                        for (int i = 0; i < B_ROWS / 64; ++i)
-                            load(sb + i * MN_BLOCK, &maps.b, n * BN + crank * B_ROWS + 64 * i, kb * BK);
+                    } else if (p.b_mn) {
+                        for (int i = 0; i < b_rows / 64; ++i)
+                            load(sb + i * MN_BLOCK, &maps.b[pi], n * bn + crank * b_rows + 64 * i, kb * BK);
                     } else {
-                        load(sb, &maps.b, kb * BK, n * BN + crank * B_ROWS);
+                        load(sb, &maps.b[pi], kb * BK, n * bn + crank * b_rows);
                     }
-                    if (++s == STAGES) {
-                        s = 0;
-                        ph ^= 1;
-                    }
+                }
+                if (++s == stages) {
+                    s = 0;
+                    ph ^= 1;
                 }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && crank == 0) {
-            constexpr uint32_t idesc = umma_idesc(1, 1, BM * PAIR, BN) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
-            // descriptor steps of 16 elements of K, in 16-byte units: 32 bytes along the swizzle row, or
-            // 16 rows of 128 bytes
-            constexpr uint64_t a_step = A_MN ? 16 * 128 / 16 : 2, b_step = B_MN ? 16 * 128 / 16 : 2;
+        if (crank == 0) {
+            const uint32_t idesc0 = umma_idesc(1, 1, BM * PAIR, bn);
             int s = 0, acc = 0;
             uint32_t ph = 0, acc_ph = 0;
             bool ok = true;
             for (int t = unit; t < num_tiles && ok; t += nunits) {
-                if (!mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, wc, SITE_TMEM_EMPTY, t)) break;
+                if (!__all_sync(0xffffffffu, mbar_wait(bar_tempty + 8 * acc, acc_ph ^ 1, wc, SITE_TMEM_EMPTY, t))) break;
                 tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * BN;
-                for (int kb = 0; kb < g.num_kb; ++kb) {
-                    if (!mbar_wait(bar_full + 8 * s, ph, wc, SITE_FULL, t)) {
+                int m, n;
+                const Product& p = g.p[tile_coords(t, g, m, n)];
+                const bool a_mn = p.a_mn != 0, b_mn = p.b_mn != 0;
+                const uint32_t idesc = idesc0 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+                // descriptor steps of 16 elements of K, in 16-byte units: 32 bytes along the swizzle row, or
+                // 16 rows of 128 bytes
+                const uint64_t a_step = a_mn ? 16 * 128 / 16 : 2, b_step = b_mn ? 16 * 128 / 16 : 2;
+                const uint32_t d_tmem = tmem_base + acc * BN_MAX;
+                for (int kb = 0; kb < p.num_kb; ++kb) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(bar_full + 8 * s, ph, wc, SITE_FULL, t))) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = ring + s * STAGE_BYTES, sb = sa + A_BYTES;
-                    const uint64_t da = A_MN ? desc_mn(sa) : umma_desc_sw128(sa);
-                    const uint64_t db = B_MN ? desc_mn(sb) : umma_desc_sw128(sb);
+                    const uint32_t sa = ring + s * stage_bytes, sb = sa + A_BYTES;
+                    const uint64_t da = a_mn ? desc_mn(sa) : umma_desc_sw128(sa);
+                    const uint64_t db = b_mn ? desc_mn(sb) : umma_desc_sw128(sb);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; ++k)
-                        umma_f16<PAIR>(d_tmem, da + a_step * k, db + b_step * k, idesc, (kb | k) != 0);
-                    // the stage is free in both CTAs once these MMAs have read it
-                    if (PAIR == 2) umma_commit_pair(bar_empty + 8 * s, 3);
-                    else umma_commit<1>(bar_empty + 8 * s);
-                    if (++s == STAGES) {
+                        for (int k = 0; k < BK / UMMA_K; ++k)
+                            umma_f16<PAIR>(d_tmem, da + a_step * k, db + b_step * k, idesc, (kb | k) != 0);
+                        // the stage is free in both CTAs once these MMAs have read it
+                        if (PAIR == 2) umma_commit_pair(bar_empty + 8 * s, 3);
+                        else umma_commit<1>(bar_empty + 8 * s);
+                    }
+                    if (++s == stages) {
                         s = 0;
                         ph ^= 1;
                     }
                 }
                 if (!ok) break;
-                if (PAIR == 2) umma_commit_pair(bar_tfull + 8 * acc, 3);
-                else umma_commit<1>(bar_tfull + 8 * acc);
+                if (elect_one()) {
+                    if (PAIR == 2) umma_commit_pair(bar_tfull + 8 * acc, 3);
+                    else umma_commit<1>(bar_tfull + 8 * acc);
+                }
                 acc ^= 1;
                 if (acc == 0) acc_ph ^= 1;
             }
@@ -282,24 +323,27 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
             return my_epi + (nbuf++ & 1) * EPI_BUF;
         };
         // `words`: bf16 units an element takes up (the maps count in those)
+        int rows = 0, cols = 0;  // of the current tile's product
         auto send = [&](uint32_t buf, const CUtensorMap* map, int col, int row, int words = 1) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-                if (col < g.N && row < g.M) tma_store_2d(map, buf, col * words, row);
+                if (col < cols && row < rows) tma_store_2d(map, buf, col * words, row);
                 tma_store_commit();
             }
         };
         for (int t = unit; t < num_tiles; t += nunits) {
             int m, n;
-            tile_coords(t, g, m, n);
+            const int pi = tile_coords(t, g, m, n);
+            rows = g.p[pi].M;
+            cols = g.p[pi].N;
             const int row0 = (m * PAIR + crank) * BM + q * 32;
             if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, acc_ph, wc, SITE_TMEM_FULL, t))) break;
             tc_fence_after();
-            const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+            const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN_MAX;
             if constexpr (EPI == EPI_STORE) {
 #pragma unroll 1
-                for (int c = 0; c < BN / 64; ++c) {
+                for (int c = 0; c < bn / 64; ++c) {
                     const uint32_t buf = next_buf();
 #pragma unroll
                     for (int hi = 0; hi < 2; ++hi) {
@@ -309,16 +353,16 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
                         pack32(f, p);
                         stage_half(buf, lane, hi, p);
                     }
-                    send(buf, &maps.out[0], n * BN + c * 64, row0);
+                    send(buf, &maps.out[pi], n * bn + c * 64, row0);
                 }
             } else if constexpr (EPI == EPI_GATED) {
 #pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    const int col = n * 128 + c * 64;
+                for (int c = 0; c < bn / 128; ++c) {
+                    const int half = bn / 2, col = n * half + c * 64;
                     if (g.save) {
 #pragma unroll 1
                         for (int part = 0; part < 4; ++part) {  // gate, up of 32 columns, gate, up of the next 32
-                            const int sub = (part & 1) * 128 + c * 64 + (part >> 1) * 32;
+                            const int sub = (part & 1) * half + c * 64 + (part >> 1) * 32;
                             const uint32_t buf = next_buf();
                             uint32_t p[32];
                             tmem_ld_32x32b_x32(t_acc + sub, p);
@@ -339,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
                         float gate[32], up[32];
                         uint32_t p[16];
                         ld_acc(t_acc + c * 64 + hi * 32, gate);
-                        ld_acc(t_acc + 128 + c * 64 + hi * 32, up);
+                        ld_acc(t_acc + half + c * 64 + hi * 32, up);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) gate[i] = gate[i] * sigmoid_f(gate[i]) * up[i];
                         pack32(gate, p);
@@ -349,27 +393,22 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
                 }
             } else {
                 const int row = row0 + lane;
-                const bool row_ok = row < g.M;
-                const float* gu = g.gu + static_cast<size_t>(row) * (2 * static_cast<size_t>(g.N));
+                const bool row_ok = row < rows;
+                const float* gu = g.gu + static_cast<size_t>(row) * (2 * static_cast<size_t>(cols));
 #pragma unroll 1
-                for (int c = 0; c < BN / 64; ++c) {
-                    const int col0 = n * BN + c * 64;
+                for (int c = 0; c < bn / 64; ++c) {
+                    const int col0 = n * bn + c * 64;
                     const uint32_t bg = next_buf();
                     uint32_t pu[2][16];
 #pragma unroll
                     for (int hi = 0; hi < 2; ++hi) {
                         const int col = col0 + hi * 32;
                         float gate[32], up[32], dh[32];
-                        ld_row32(gu + col, col, g.N, row_ok, gate);
-                        ld_row32(gu + g.N + col, col, g.N, row_ok, up);
+                        ld_row32(gu + col, col, cols, row_ok, gate);
+                        ld_row32(gu + cols + col, col, cols, row_ok, up);
                         ld_acc(t_acc + c * 64 + hi * 32, dh);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float s = sigmoid_f(gate[i]);
-                            const float d = dh[i];
-                            dh[i] = d * gate[i] * s;                                          // du
-                            gate[i] = d * up[i] * s * (1.0f + gate[i] * (1.0f - s));          // dg
-                        }
+                        for (int i = 0; i < 32; ++i) d_gated(dh[i], gate[i], up[i], gate[i], dh[i]);
                         uint32_t pg[16];
                         pack32(gate, pg);
                         stage_half(bg, lane, hi, pg);
@@ -418,9 +457,11 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
 // of S CTAs until there are enough CTAs to draw on all of HBM. Each CTA leaves its fp32 partial sums in its own
 // shared memory; the cluster's CTAs then add up each other's through distributed shared memory, in rank order: no
 // workspace, no second launch, the same bits on every run.
-//   GATED: a tile is 64 gate rows and the 64 up rows of the same columns; silu(g) * u leaves.
-// The second product (from h) may start while the first still runs: its weights do not depend on the first, so the
-// ring is filled with them, and only then does it wait for the rows of h.
+//   EPI_GATED   a tile is 64 gate rows and the 64 up rows of the same columns; silu(g) * u leaves as h
+//   EPI_STORE   y from h and W2, or dx from [dg|du] and W13 (MN-major: 128 columns of W13)
+//   EPI_DGATED  dh from dy and W2 (MN-major: 128 columns of W2), with the kept g, u straight into dg, du
+// A product that follows another of the same call may start while that one still runs: its weights do not depend
+// on it, so the ring is filled with them, and only then does it wait for the rows it reads.
 constexpr int ROWS_THREADS = 192;
 template <int N>
 struct RowsCfg {
@@ -437,9 +478,9 @@ struct RowsMaps {
     CUtensorMap w, x;
 };
 struct RowsArgs {
-    int T, cols, num_kb;  // cols: columns of the output (F or H)
-    __nv_bfloat16* out;   // [T, cols]
-    float* gu;            // GATED: [T, 2 cols], may be null
+    int T, cols, num_kb;  // cols: columns of the output (GATED, DGATED: F)
+    __nv_bfloat16* out;   // [T, cols]; DGATED: [T, 2 cols]
+    float* gu;            // [T, 2 cols]; GATED: written, may be null; DGATED: read
     unsigned* status;
 };
 __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
@@ -448,9 +489,10 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
     return v;
 }
 
-template <bool GATED, int N>
+template <int EPI, bool W_MN, int N>
 __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsArgs g) {
     using C = RowsCfg<N>;
+    constexpr bool GATED = EPI == EPI_GATED;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t ctrl = ring + C::STAGES * C::STAGE;
@@ -488,69 +530,84 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    // the next kernel's CTAs may take the places that this one's leave
-    if (GATED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    auto meet = [&]() {  // of the cluster's CTAs, every thread of them
+        if (S == 1) {
+            __syncthreads();
+        } else {
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+        }
+    };
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // as in ffn_gemm_kernel
 
-    if (warp == 0) {
-        if (lane == 0) {
-            auto load_w = [&](int kb, int s) {
-                const uint32_t sw = ring + s * C::STAGE, full = bar_full + 8 * s;
-                mbar_expect_tx(full, C::STAGE);
-                if (GATED) {
-                    // gate rows that do not exist read up rows instead, up rows zeros: not stored
-                    tma_load_2d(sw, &maps.w, full, kb * BK, tile * 64);
-                    tma_load_2d(sw + C::W_BYTES / 2, &maps.w, full, kb * BK, g.cols + tile * 64);
-                } else {
-                    tma_load_2d(sw, &maps.w, full, kb * BK, tile * 128);
-                }
-            };
-            auto load_x = [&](int kb, int s) {
-                tma_load_2d(ring + s * C::STAGE + C::W_BYTES, &maps.x, bar_full + 8 * s, kb * BK, tok0);
-            };
-            const int ahead = min(kb1 - kb0, C::STAGES);
-            for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
-            if (!GATED) {
-                // h is complete and visible from here on, to the copy engine too
-                asm volatile("griddepcontrol.wait;" ::: "memory");
-                asm volatile("fence.proxy.async;" ::: "memory");
+    if (warp == 0) {  // whole warps, one elected thread: as in ffn_gemm_kernel
+        auto load_w = [&](int kb, int s) {
+            const uint32_t sw = ring + s * C::STAGE, full = bar_full + 8 * s;
+            mbar_expect_tx(full, C::STAGE);
+            if (GATED) {
+                // gate rows that do not exist read up rows instead, up rows zeros: not stored
+                tma_load_2d(sw, &maps.w, full, kb * BK, tile * 64);
+                tma_load_2d(sw + C::W_BYTES / 2, &maps.w, full, kb * BK, g.cols + tile * 64);
+            } else if (W_MN) {
+                tma_load_2d(sw, &maps.w, full, tile * 128, kb * BK);
+                tma_load_2d(sw + MN_BLOCK, &maps.w, full, tile * 128 + 64, kb * BK);
+            } else {
+                tma_load_2d(sw, &maps.w, full, kb * BK, tile * 128);
             }
+        };
+        auto load_x = [&](int kb, int s) {
+            tma_load_2d(ring + s * C::STAGE + C::W_BYTES, &maps.x, bar_full + 8 * s, kb * BK, tok0);
+        };
+        const int ahead = min(kb1 - kb0, C::STAGES);
+        if (elect_one()) {
+            for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
+        }
+        // what the kernel before wrote is complete and visible from here on, to the copy engine too
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("fence.proxy.async;" ::: "memory");
+        if (elect_one()) {
             for (int i = 0; i < ahead; ++i) load_x(kb0 + i, i);
-            int s = 0;
-            uint32_t ph = 0;
-            for (int kb = kb0 + ahead; kb < kb1; ++kb) {
-                if (!mbar_wait(bar_empty + 8 * s, ph, wc, SITE_EMPTY, tile)) break;
+        }
+        int s = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0 + ahead; kb < kb1; ++kb) {
+            if (!__all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * s, ph, wc, SITE_EMPTY, tile))) break;
+            if (elect_one()) {
                 load_w(kb, s);
                 load_x(kb, s);
-                if (++s == C::STAGES) {
-                    s = 0;
-                    ph ^= 1;
-                }
+            }
+            if (++s == C::STAGES) {
+                s = 0;
+                ph ^= 1;
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = umma_idesc(1, 1, 128, N);
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait(bar_full + 8 * s, ph, wc, SITE_FULL, tile)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint64_t da = umma_desc_sw128(ring + s * C::STAGE);
-                const uint64_t db = umma_desc_sw128(ring + s * C::STAGE + C::W_BYTES);
-#pragma unroll
-                for (int k = 0; k < BK / UMMA_K; ++k) umma_f16<1>(tmem, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
-                umma_commit<1>(bar_empty + 8 * s);
-                if (++s == C::STAGES) {
-                    s = 0;
-                    ph ^= 1;
-                }
+        constexpr uint32_t idesc = umma_idesc(1, 1, 128, N) | (W_MN ? 1u << 15 : 0u);
+        constexpr uint64_t w_step = W_MN ? 16 * 128 / 16 : 2;
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (!__all_sync(0xffffffffu, mbar_wait(bar_full + 8 * s, ph, wc, SITE_FULL, tile))) {
+                ok = false;
+                break;
             }
-            if (ok) umma_commit<1>(bar_done);
+            tc_fence_after();
+            const uint64_t da = W_MN ? desc_mn(ring + s * C::STAGE) : umma_desc_sw128(ring + s * C::STAGE);
+            const uint64_t db = umma_desc_sw128(ring + s * C::STAGE + C::W_BYTES);
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < BK / UMMA_K; ++k)
+                    umma_f16<1>(tmem, da + w_step * k, db + 2 * k, idesc, kb != kb0 || k != 0);
+                umma_commit<1>(bar_empty + 8 * s);
+            }
+            if (++s == C::STAGES) {
+                s = 0;
+                ph ^= 1;
+            }
         }
+        if (ok && elect_one()) umma_commit<1>(bar_done);
     } else {
         // partial sums as [token][weight row]; every load has been consumed, so the ring is free
         const int q = warp & 3;
@@ -571,46 +628,76 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
         }
     }
     tc_fence_before();
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
+    meet();
     {
         constexpr int PAIRS = GATED ? 32 : 64;  // pairs of neighbouring output columns of a tile
         const int count = min(N, g.T - tok0) * PAIRS;
-        for (int e = rank * ROWS_THREADS + threadIdx.x; e < count; e += S * ROWS_THREADS) {
-            const int n = e / PAIRS, p = e % PAIRS;
-            const int col = tile * (2 * PAIRS) + 2 * p;
-            const uint32_t at = ring + (n * 128 + 2 * p) * 4;
-            float2 a = make_float2(0.f, 0.f), b = make_float2(0.f, 0.f);
+        // U elements a turn, so that their loads (a peer's shared memory, the kept g and u) are in flight together
+        constexpr int U = 4;
+        const int step = S * ROWS_THREADS;
+        for (int e0 = rank * ROWS_THREADS + threadIdx.x; e0 < count; e0 += U * step) {
+            float2 a[U], b[U], gate[U], up[U];
+            uint32_t at[U];
+            size_t place[U];  // of the output, and of g in [g|u]
+            bool ok[U];
+            const size_t wide = EPI == EPI_STORE ? g.cols : 2 * static_cast<size_t>(g.cols);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int e = e0 + i * step, n = e / PAIRS, p = e % PAIRS;
+                const int col = tile * (2 * PAIRS) + 2 * p;
+                ok[i] = e < count && col < g.cols;
+                at[i] = ring + (n * 128 + 2 * p) * 4;
+                place[i] = static_cast<size_t>(tok0 + n) * wide + col;
+                a[i] = make_float2(0.f, 0.f);
+                b[i] = make_float2(0.f, 0.f);
+                if (EPI == EPI_DGATED && ok[i]) {
+                    gate[i] = *reinterpret_cast<const float2*>(g.gu + place[i]);
+                    up[i] = *reinterpret_cast<const float2*>(g.gu + place[i] + g.cols);
+                }
+            }
             for (int s = 0; s < S; ++s) {
-                const uint32_t peer = mapa_shared(at, s);
-                const float2 v = ld_cluster_f2(peer);
-                a.x += v.x;
-                a.y += v.y;
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    if (!ok[i]) continue;
+                    const uint32_t peer = mapa_shared(at[i], s);
+                    const float2 v = ld_cluster_f2(peer);
+                    a[i].x += v.x;
+                    a[i].y += v.y;
+                    if (GATED) {
+                        const float2 u = ld_cluster_f2(peer + 64 * 4);
+                        b[i].x += u.x;
+                        b[i].y += u.y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (!ok[i]) continue;
+                if (EPI == EPI_DGATED) {
+                    float2 dg, du;
+                    d_gated(a[i].x, gate[i].x, up[i].x, dg.x, du.x);
+                    d_gated(a[i].y, gate[i].y, up[i].y, dg.y, du.y);
+                    *reinterpret_cast<uint32_t*>(g.out + place[i]) = pack_bf16x2(dg.x, dg.y);
+                    *reinterpret_cast<uint32_t*>(g.out + place[i] + g.cols) = pack_bf16x2(du.x, du.y);
+                    continue;
+                }
+                size_t to = place[i];
                 if (GATED) {
-                    const float2 u = ld_cluster_f2(peer + 64 * 4);
-                    b.x += u.x;
-                    b.y += u.y;
+                    if (g.gu != nullptr) {
+                        *reinterpret_cast<float2*>(g.gu + place[i]) = a[i];
+                        *reinterpret_cast<float2*>(g.gu + place[i] + g.cols) = b[i];
+                    }
+                    a[i].x = a[i].x * sigmoid_f(a[i].x) * b[i].x;
+                    a[i].y = a[i].y * sigmoid_f(a[i].y) * b[i].y;
+                    const int n = (e0 + i * step) / PAIRS;
+                    to -= static_cast<size_t>(tok0 + n) * g.cols;  // h has rows of half that width
                 }
+                *reinterpret_cast<uint32_t*>(g.out + to) = pack_bf16x2(a[i].x, a[i].y);
             }
-            if (col >= g.cols) continue;
-            const size_t row = static_cast<size_t>(tok0 + n);
-            if (GATED) {
-                if (g.gu != nullptr) {
-                    float* gu = g.gu + row * (2 * static_cast<size_t>(g.cols)) + col;
-                    *reinterpret_cast<float2*>(gu) = a;
-                    *reinterpret_cast<float2*>(gu + g.cols) = b;
-                }
-                a.x = a.x * sigmoid_f(a.x) * b.x;
-                a.y = a.y * sigmoid_f(a.y) * b.y;
-            }
-            *reinterpret_cast<uint32_t*>(g.out + row * g.cols + col) = pack_bf16x2(a.x, a.y);
         }
     }
     // a CTA's partial sums stay until every peer has read them
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
+    meet();
     if (warp == 1) {
         tc_fence_after();
         if (*abort_sm) {
@@ -631,121 +718,182 @@ static int operand_map(CUtensorMap* map, const void* p, bool mn, int rows_or_col
     return make_tmap_2d(map, p, 2, K, rows_or_cols, static_cast<uint64_t>(K) * 2, BK, box);
 }
 
-template <bool A_MN, bool B_MN, int EPI, int PAIR>
-static int launch(const Maps& maps, const Args& g, cudaStream_t st) {
-    const auto kernel = ffn_gemm_kernel<A_MN, B_MN, EPI, PAIR>;
-    static bool attr_set[64] = {false};
-    int dev = 0, sms = 0;
-    DK_CUDA_OK(cudaGetDevice(&dev));
-    if (!attr_set[dev & 63]) {
-        DK_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<PAIR>::SMEM_BYTES));
-        attr_set[dev & 63] = true;
-    }
-    const int rc = sm_count(&sms);
-    if (rc != DK_OK) return rc;
-    const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
-    const int units = sms / PAIR;
+// Launch attributes: the cluster's size, and (`follows`) the permission to start while the kernel before it on the
+// stream, which is one of the same call, still runs.
+struct Launch {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<int>(tiles < units ? tiles : units) * PAIR);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Cfg<PAIR>::SMEM_BYTES;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = PAIR;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    DK_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, maps, g));
+    cudaLaunchAttribute attr[2];
+    Launch(dim3 grid, int threads, int smem, int cluster, bool follows, cudaStream_t st) {
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = cluster;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = follows ? 2 : 1;
+    }
+};
+template <typename K>
+static int allow_smem(K kernel, int bytes, bool (&done)[64]) {
+    int dev = 0;
+    DK_CUDA_OK(cudaGetDevice(&dev));
+    if (!done[dev & 63]) {
+        DK_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done[dev & 63] = true;
+    }
     return DK_OK;
 }
 
-// Two-CTA tiles unless more than one row tile in nine would be computed for nothing.
-static bool use_pair(int M) {
-    const int tiles = (M + BM - 1) / BM;
-    return tiles % 2 == 0 || tiles >= 9;
+template <int EPI, int PAIR>
+static int launch(const Maps& maps, const Args& g, bool follows, cudaStream_t st) {
+    const auto kernel = ffn_gemm_kernel<EPI, PAIR>;
+    static bool done[64] = {false};
+    int sms = 0;
+    int rc = allow_smem(kernel, SMEM_BYTES, done);
+    if (rc == DK_OK) rc = sm_count(&sms);
+    if (rc != DK_OK) return rc;
+    const int units = sms / PAIR;
+    Launch l(dim3((g.num_tiles < units ? g.num_tiles : units) * PAIR), THREADS, SMEM_BYTES, PAIR, follows, st);
+    DK_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, maps, g));
+    return DK_OK;
 }
 
-// D[M,N] = A B. GATED: B = W13 [2N, K], D = h. DGATED: D = dgu [M, 2N].
-template <bool A_MN, bool B_MN, int EPI>
-static int product(const void* A, const void* B, void* D, int M, int N, int K, void* gu, cudaStream_t st) {
+// One product: D[M,N] = A B. GATED: B = W13 [2N, K], D = h; DGATED: D = dgu [M, 2N].
+struct Spec {
+    const void *A, *B;
+    void* D;
+    int M, N, K;
+    bool a_mn, b_mn;
+};
+
+// How the products of a launch are tiled. A tile's time is its K blocks, each as long as measured with all SMs at work
+// (in units of a pair's 256 columns, 0.335 us), and its epilogue, overlapped with the next tile's K blocks:
+//   two CTAs    256 columns 1.0   192 columns 0.85   128 columns 0.8
+//   one CTA     256 columns 1.1   192 columns 0.95   128 columns 0.75
+// Wide pairs are fastest per flop (they load least per flop; 128 columns are bound by L2); narrow tiles and single CTAs cut
+// the work finer where it would not go evenly into waves, or compute fewer rows for nothing. 192 columns only where
+// nothing but a K-major B is loaded and stored.
+struct Tiling {
+    int pair, bn;
+};
+static Tiling choose(const Spec* s, int count, int epi, int sms) {
+    static const double block[2][3] = {{0.75, 0.95, 1.1}, {0.8, 0.85, 1.0}};
+    Tiling best{1, 256};
+    double least = 1e300;
+    for (int pair = 1; pair <= 2; ++pair)
+        for (int bn = 256; bn >= 128; bn -= 64) {
+            bool allowed = true;
+            double work = 0, longest = 0;
+            int64_t tiles = 0;
+            const double epilogue = bn * (epi == EPI_STORE ? 0.02 : 0.04);
+            for (int i = 0; i < count; ++i) {
+                if (bn == 192 && (epi != EPI_STORE || s[i].b_mn)) allowed = false;
+                const int rows = BM * pair, cols = epi == EPI_GATED ? bn / 2 : bn;
+                const int64_t n = static_cast<int64_t>((s[i].M + rows - 1) / rows) * ((s[i].N + cols - 1) / cols);
+                double one = ((s[i].K + BK - 1) / BK) * block[pair - 1][bn / 64 - 2];
+                if (one < epilogue) one = epilogue;
+                work += n * one;
+                tiles += n;
+                if (one > longest) longest = one;
+            }
+            if (!allowed) continue;
+            const int units = sms / pair;
+            // equal tiles go in whole waves, a mix of them evenly
+            const double time = (count == 1 ? ((tiles + units - 1) / units) * longest
+                                            : (tiles <= units ? longest : work / units + 0.5 * longest)) + epilogue;
+            if (time < least) {
+                least = time;
+                best = Tiling{pair, bn};
+            }
+        }
+    return best;
+}
+
+// gu: GATED: where g and u go (may be null); DGATED: where they come from
+template <int EPI>
+static int products(const Spec* s, int count, void* gu, bool follows, cudaStream_t st) {
+    int sms = 0;
+    int rc = sm_count(&sms);
+    if (rc != DK_OK) return rc;
+    const Tiling t = choose(s, count, EPI, sms);
     Maps maps;
     Args g{};
-    const int pair = use_pair(M) ? 2 : 1;
-    int rc = operand_map(&maps.a, A, A_MN, M, K, BM);
-    if (rc != DK_OK) return rc;
-    rc = operand_map(&maps.b, B, B_MN, EPI == EPI_GATED ? 2 * N : N, K, EPI == EPI_GATED ? 128 : BN / pair);
-    if (rc != DK_OK) return rc;
-    // a map counts bf16 units: `words` of them to an element
-    auto out = [&](int i, void* p, uint64_t stride, int words) {
-        return make_tmap_2d(&maps.out[i], p, 2, static_cast<uint64_t>(N) * words, M, stride, 64, 32);
-    };
-    const uint64_t n = static_cast<uint64_t>(N);
-    if (EPI == EPI_DGATED) {
-        rc = out(0, D, 4 * n, 1);
-        if (rc == DK_OK) rc = out(1, static_cast<__nv_bfloat16*>(D) + n, 4 * n, 1);
-    } else {
-        rc = out(0, D, 2 * n, 1);
-        if (EPI == EPI_GATED && gu != nullptr) {
-            if (rc == DK_OK) rc = out(1, gu, 8 * n, 2);
-            if (rc == DK_OK) rc = out(2, static_cast<float*>(gu) + n, 8 * n, 2);
+    for (int i = 0; i < count && rc == DK_OK; ++i) {
+        Product& p = g.p[i];
+        const int bn_out = EPI == EPI_GATED ? t.bn / 2 : t.bn;
+        p.M = s[i].M;
+        p.N = s[i].N;
+        p.num_kb = (s[i].K + BK - 1) / BK;
+        p.tiles_m = (p.M + BM * t.pair - 1) / (BM * t.pair);
+        p.tiles_n = (p.N + bn_out - 1) / bn_out;
+        p.group_m = 16 / t.pair;
+        p.first = g.num_tiles;
+        p.a_mn = s[i].a_mn;
+        p.b_mn = s[i].b_mn;
+        const int64_t all = g.num_tiles + static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+        DK_REQUIRE(all < (1 << 30), "too many tiles");
+        g.num_tiles = static_cast<int>(all);
+        rc = operand_map(&maps.a[i], s[i].A, s[i].a_mn, p.M, s[i].K, BM);
+        if (rc == DK_OK)
+            rc = operand_map(&maps.b[i], s[i].B, s[i].b_mn, EPI == EPI_GATED ? 2 * p.N : p.N, s[i].K,
+                             EPI == EPI_GATED ? t.bn / 2 : t.bn / t.pair);
+        // a map counts bf16 units: `words` of them to an element
+        auto out = [&](int j, void* d, uint64_t stride, int words) {
+            if (rc == DK_OK)
+                rc = make_tmap_2d(&maps.out[j], d, 2, static_cast<uint64_t>(p.N) * words, p.M, stride, 64, 32);
+        };
+        const uint64_t n = static_cast<uint64_t>(p.N);
+        if (EPI == EPI_DGATED) {
+            out(0, s[i].D, 4 * n, 1);
+            out(1, static_cast<__nv_bfloat16*>(s[i].D) + n, 4 * n, 1);
+        } else {
+            out(i, s[i].D, 2 * n, 1);
+            if (EPI == EPI_GATED && gu != nullptr) {
+                out(1, gu, 8 * n, 2);
+                out(2, static_cast<float*>(gu) + n, 8 * n, 2);
+            }
         }
     }
     if (rc != DK_OK) return rc;
-    g.M = M;
-    g.N = N;
-    g.num_kb = (K + BK - 1) / BK;
-    g.tiles_m = (M + BM * pair - 1) / (BM * pair);
-    g.tiles_n = (N + (EPI == EPI_GATED ? 128 : BN) - 1) / (EPI == EPI_GATED ? 128 : BN);
-    g.group_m = 16 / pair;
+    g.products = count;
+    g.bn = t.bn;
     g.save = EPI == EPI_GATED && gu != nullptr;
     g.gu = static_cast<const float*>(gu);
     rc = device_status_ptr(&g.status);
     if (rc != DK_OK) return rc;
-    return pair == 2 ? launch<A_MN, B_MN, EPI, 2>(maps, g, st) : launch<A_MN, B_MN, EPI, 1>(maps, g, st);
+    return t.pair == 2 ? launch<EPI, 2>(maps, g, follows, st) : launch<EPI, 1>(maps, g, follows, st);
 }
 
-template <bool GATED, int N>
-static int launch_rows(const RowsMaps& maps, const RowsArgs& g, int tiles, int S, cudaStream_t st) {
-    using C = RowsCfg<N>;
-    const auto kernel = ffn_rows_kernel<GATED, N>;
-    static bool attr_set[64] = {false};
-    int dev = 0;
-    DK_CUDA_OK(cudaGetDevice(&dev));
-    if (!attr_set[dev & 63]) {
-        DK_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
-        attr_set[dev & 63] = true;
-    }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(tiles * S, (g.T + N - 1) / N);
-    cfg.blockDim = dim3(ROWS_THREADS);
-    cfg.dynamicSmemBytes = C::SMEM_BYTES;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = S;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    // the second product overlaps the end of the first, which is the kernel before it on the stream
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = GATED ? 1 : 2;
-    DK_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, maps, g));
+template <int EPI, bool W_MN, int N>
+static int launch_rows(const RowsMaps& maps, const RowsArgs& g, int tiles, int S, bool follows, cudaStream_t st) {
+    const auto kernel = ffn_rows_kernel<EPI, W_MN, N>;
+    static bool done[64] = {false};
+    const int rc = allow_smem(kernel, RowsCfg<N>::SMEM_BYTES, done);
+    if (rc != DK_OK) return rc;
+    Launch l(dim3(tiles * S, (g.T + N - 1) / N), ROWS_THREADS, RowsCfg<N>::SMEM_BYTES, S, follows, st);
+    DK_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, maps, g));
     return DK_OK;
 }
 
-// out [T, cols] = x W^T for few rows; GATED: W = W13, out = h
-template <bool GATED>
-static int rows_product(const void* x, const void* W, void* out, int T, int cols, int K, void* gu, cudaStream_t st) {
+static int rows_tokens(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256; }
+
+// out [T, cols] = x W^T for few rows. GATED: W = W13, out = h; DGATED: x = dy, out = dgu. W_MN: W is [K, cols].
+template <int EPI, bool W_MN>
+static int rows_product(const void* x, const void* W, void* out, int T, int cols, int K, void* gu, bool follows,
+                        cudaStream_t st) {
     int sms = 0;
     int rc = sm_count(&sms);
     if (rc != DK_OK) return rc;
-    const int N = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+    const bool gated = EPI == EPI_GATED;
+    const int N = rows_tokens(T);
     RowsMaps maps;
-    rc = make_tmap_2d(&maps.w, W, 2, K, GATED ? 2 * cols : cols, static_cast<uint64_t>(K) * 2, BK, GATED ? 64 : 128);
-    if (rc == DK_OK) rc = make_tmap_2d(&maps.x, x, 2, K, T, static_cast<uint64_t>(K) * 2, BK, N);
+    rc = operand_map(&maps.w, W, W_MN, gated ? 2 * cols : cols, K, gated ? 64 : 128);
+    if (rc == DK_OK) rc = operand_map(&maps.x, x, false, T, K, N);
     if (rc != DK_OK) return rc;
     RowsArgs g{};
     g.T = T;
@@ -755,17 +903,17 @@ static int rows_product(const void* x, const void* W, void* out, int T, int cols
     g.gu = static_cast<float*>(gu);
     rc = device_status_ptr(&g.status);
     if (rc != DK_OK) return rc;
-    const int tiles = (cols + (GATED ? 64 : 128) - 1) / (GATED ? 64 : 128);
+    const int tiles = (cols + (gated ? 64 : 128) - 1) / (gated ? 64 : 128);
     // cut K while the CTAs still run all at once and each keeps a few K blocks
     const int places = sms * (N <= 128 ? 2 : 1);
     int S = 1;
-    while (S < 8 && tiles * S * 2 * ((T + N - 1) / N) <= places && g.num_kb / (S * 2) >= 4) S *= 2;
+    while (S < 8 && tiles * S * 2 * ((T + N - 1) / N) <= places && g.num_kb / (S * 2) >= 2) S *= 2;
     switch (N) {
-        case 16: return launch_rows<GATED, 16>(maps, g, tiles, S, st);
-        case 32: return launch_rows<GATED, 32>(maps, g, tiles, S, st);
-        case 64: return launch_rows<GATED, 64>(maps, g, tiles, S, st);
-        case 128: return launch_rows<GATED, 128>(maps, g, tiles, S, st);
-        default: return launch_rows<GATED, 256>(maps, g, tiles, S, st);
+        case 16: return launch_rows<EPI, W_MN, 16>(maps, g, tiles, S, follows, st);
+        case 32: return launch_rows<EPI, W_MN, 32>(maps, g, tiles, S, follows, st);
+        case 64: return launch_rows<EPI, W_MN, 64>(maps, g, tiles, S, follows, st);
+        case 128: return launch_rows<EPI, W_MN, 128>(maps, g, tiles, S, follows, st);
+        default: return launch_rows<EPI, W_MN, 256>(maps, g, tiles, S, follows, st);
     }
 }
 
@@ -776,6 +924,13 @@ static int check_shape(int T, int H, int F) {
     DK_REQUIRE(T >= 0, "the number of rows must not be negative");
     DK_REQUIRE(H >= 8 && F >= 8 && H % 8 == 0 && F % 8 == 0, "H and F must be positive multiples of 8");
     DK_REQUIRE(T <= (1 << 24) && H <= (1 << 20) && F <= (1 << 20), "at most 2^24 rows and widths of 2^20");
+    return DK_OK;
+}
+
+static int check_aligned(std::initializer_list<const void*> ps) {
+    uintptr_t bits = 0;
+    for (const void* p : ps) bits |= reinterpret_cast<uintptr_t>(p);
+    DK_REQUIRE((bits & 15) == 0, "every tensor must be 16-byte aligned");
     return DK_OK;
 }
 
@@ -792,16 +947,17 @@ extern "C" int dk_gated_ffn(const void* x, const void* w13, const void* w2, int 
     if (T == 0) return DK_OK;
     DK_REQUIRE(x != nullptr && h != nullptr && y != nullptr, "null operand");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    DK_REQUIRE(((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(gu)) & 15) == 0,
-               "h, y and gu must be 16-byte aligned");
-    if (T <= ROWS_MAX_T) {
-        rc = rows_product<true>(x, w13, h, T, F, H, gu, st);
-        if (rc != DK_OK) return rc;
-        return rows_product<false>(h, w2, y, T, H, F, nullptr, st);
-    }
-    rc = product<false, false, EPI_GATED>(x, w13, h, T, F, H, gu, st);
+    rc = check_aligned({x, w13, w2, gu, h, y});
     if (rc != DK_OK) return rc;
-    return product<false, false, EPI_STORE>(h, w2, y, T, H, F, nullptr, st);
+    if (T <= ROWS_MAX_T) {
+        rc = rows_product<EPI_GATED, false>(x, w13, h, T, F, H, gu, false, st);
+        if (rc != DK_OK) return rc;
+        return rows_product<EPI_STORE, false>(h, w2, y, T, H, F, nullptr, true, st);
+    }
+    const Spec up{x, w13, h, T, F, H, false, false}, down{h, w2, y, T, H, F, false, false};
+    rc = products<EPI_GATED>(&up, 1, gu, false, st);
+    if (rc != DK_OK) return rc;
+    return products<EPI_STORE>(&down, 1, nullptr, true, st);
 }
 
 extern "C" int dk_gated_ffn_bwd(const void* dy, const void* x, const void* w13, const void* w2, const void* gu, const void* h,
@@ -817,12 +973,29 @@ extern "C" int dk_gated_ffn_bwd(const void* dy, const void* x, const void* w13, 
         DK_CUDA_OK(cudaMemsetAsync(dw2, 0, static_cast<size_t>(F) * H * 2, st));
         return DK_OK;
     }
-    DK_REQUIRE((reinterpret_cast<uintptr_t>(gu) & 15) == 0, "gu must be 16-byte aligned");
     DK_REQUIRE(dy != nullptr && x != nullptr && gu != nullptr && h != nullptr && dgu != nullptr && dx != nullptr, "null operand");
-    // dh = dy W2 (K = H, W2 [H,F] is [K,N]), straight into dg and du
-    rc = product<false, true, EPI_DGATED>(dy, w2, dgu, T, F, H, const_cast<void*>(gu), st);
-    if (rc == DK_OK) rc = product<false, true, EPI_STORE>(dgu, w13, dx, T, H, 2 * F, nullptr, st);
-    if (rc == DK_OK) rc = product<true, true, EPI_STORE>(dgu, x, dw13, 2 * F, H, T, nullptr, st);
-    if (rc == DK_OK) rc = product<true, true, EPI_STORE>(dy, h, dw2, H, F, T, nullptr, st);
+    rc = check_aligned({dy, x, w13, w2, gu, h, dgu, dx, dw13, dw2});
+    if (rc != DK_OK) return rc;
+    // dW13 [2F,H] = dgu^T x and dW2 [H,F] = dy^T h, the tokens as K
+    const Spec d_w13{dgu, x, dw13, 2 * F, H, T, true, true}, d_w2{dy, h, dw2, H, F, T, true, true};
+    if (T <= ROWS_MAX_T) {
+        // dh = dy W2 straight into dg and du, then dx = dgu W13
+        rc = rows_product<EPI_DGATED, true>(dy, w2, dgu, T, F, H, const_cast<void*>(gu), false, st);
+        if (rc == DK_OK) rc = rows_product<EPI_STORE, true>(dgu, w13, dx, T, H, 2 * F, nullptr, true, st);
+        const Spec two[2] = {d_w13, d_w2};
+        if (rc == DK_OK) rc = products<EPI_STORE>(two, 2, nullptr, true, st);
+        return rc;
+    }
+    const Spec d_h{dy, w2, dgu, T, F, H, false, true}, d_x{dgu, w13, dx, T, H, 2 * F, false, true};
+    rc = products<EPI_DGATED>(&d_h, 1, const_cast<void*>(gu), false, st);
+    if (rc != DK_OK) return rc;
+    // the longest tiles first
+    Spec three[3] = {d_x, d_w13, d_w2};
+    if (T > 2 * F) {
+        three[0] = d_w13;
+        three[1] = d_w2;
+        three[2] = d_x;
+    }
+    rc = products<EPI_STORE>(three, 3, nullptr, true, st);
     return rc;
 }

@@ -63,12 +63,14 @@ def test_c_abi_argument_errors(capi):
     assert bad == [capi.ERR_ARG] * len(bad)
     ffn = lambda T=4, H=64, F=32, x=one, w13=one, w2=one, h=one, y=one: L.dk_gated_ffn(x, w13, w2, T, H, F, None, h, y, None)
     bad = [ffn(T=-1), ffn(H=0), ffn(F=0), ffn(H=60), ffn(F=20), ffn(x=None), ffn(w13=None), ffn(w2=None), ffn(h=None), ffn(y=None),
-           ffn(T=(1 << 24) + 1), ffn(H=(1 << 20) + 8)]
+           ffn(T=(1 << 24) + 1), ffn(H=(1 << 20) + 8), ffn(x=_p(4104)), ffn(w2=_p(4100)), ffn(y=_p(4104))]
     assert bad == [capi.ERR_ARG] * len(bad)
     assert ffn(T=0, x=None, h=None, y=None) == 0
     for k in range(10):
         args = [one] * 6 + [4, 64, 32] + [one] * 4
         args[k if k < 6 else k + 3] = None
+        assert L.dk_gated_ffn_bwd(*args, None) == capi.ERR_ARG, k
+        args[k if k < 6 else k + 3] = _p(4104)
         assert L.dk_gated_ffn_bwd(*args, None) == capi.ERR_ARG, k
 
 
