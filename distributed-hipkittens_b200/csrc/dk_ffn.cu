@@ -35,6 +35,7 @@
 #include "dk_host.h"
 #include "dk_ptx.cuh"
 
+#include <algorithm>
 #include <initializer_list>
 
 namespace dk {
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
 
 // --------------------------------------------------------------------------------------------
 // Few rows (single tokens, batches of sequences being answered): bound by reading the weights once. The roles are
-// swapped: 128 weight rows are the tensor core's M, the tokens its N (padded to 16..256), so a tile is 16 KB of
+// swapped: 128 weight rows are the tensor core's M, the tokens its N (16 to 256, in steps of 16), so a tile is 16 KB of
 // weights per 64 of K whatever the number of tokens, and F / 64 or H / 128 tiles are cut along K over a cluster
 // of S CTAs until there are enough CTAs to draw on all of HBM. Each CTA leaves its fp32 partial sums in its own
 // shared memory; the cluster's CTAs then add up each other's through distributed shared memory, in rank order: no
@@ -463,21 +464,17 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
 // A product that follows another of the same call may start while that one still runs: its weights do not depend
 // on it, so the ring is filled with them, and only then does it wait for the rows it reads.
 constexpr int ROWS_THREADS = 192;
-template <int N>
-struct RowsCfg {
-    static constexpr int W_BYTES = 128 * BK * 2;
-    static constexpr int STAGE = W_BYTES + N * BK * 2;
-    // two CTAs per SM up to 128 tokens, one for 256
-    static constexpr int STAGES = N <= 32 ? 5 : N == 64 ? 4 : N == 128 ? 3 : 4;
-    static constexpr int CTAS_PER_SM = N <= 128 ? 2 : 1;
-    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE + 128;
-    static constexpr int TMEM = N < 32 ? 32 : N;
-    static_assert(N * 128 * 4 <= STAGES * STAGE, "the partial sums reuse the ring");
-};
+constexpr int ROWS_W_BYTES = 128 * BK * 2;
+// Shared memory of the ring: two CTAs on an SM up to 128 tokens, one above. The partial sums reuse it: N * 512 bytes.
+constexpr int ROWS_MAX_STAGES = 8;
+__host__ __device__ constexpr int rows_ring(int N) { return N <= 128 ? 110 * 1024 : 208 * 1024; }
+constexpr int rows_smem(int N) { return 1024 + rows_ring(N) + 256; }
+static_assert(128 * 512 <= rows_ring(128) && 256 * 512 <= rows_ring(256), "the partial sums reuse the ring");
 struct RowsMaps {
     CUtensorMap w, x;
 };
 struct RowsArgs {
+    int N;                // tokens of a tile, a multiple of 16
     int T, cols, num_kb;  // cols: columns of the output (GATED, DGATED: F)
     __nv_bfloat16* out;   // [T, cols]; DGATED: [T, 2 cols]
     float* gu;            // [T, 2 cols]; GATED: written, may be null; DGATED: read
@@ -489,17 +486,18 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
     return v;
 }
 
-template <int EPI, bool W_MN, int N>
+template <int EPI, bool W_MN>
 __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsArgs g) {
-    using C = RowsCfg<N>;
+    const int N = g.N, stage = ROWS_W_BYTES + N * BK * 2, stages = min(ROWS_MAX_STAGES, rows_ring(N) / stage);
+    const int tmem_cols = N <= 32 ? 32 : N <= 64 ? 64 : N <= 128 ? 128 : 256;  // a power of two
     constexpr bool GATED = EPI == EPI_GATED;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t ctrl = ring + C::STAGES * C::STAGE;
+    const uint32_t ctrl = ring + rows_ring(N);
     uint8_t* ctrl_p = smem_raw + (ctrl - smem_u32(smem_raw));
-    const uint32_t bar_full = ctrl, bar_empty = ctrl + 8 * C::STAGES, bar_done = ctrl + 16 * C::STAGES;
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl_p + 16 * C::STAGES + 8);
-    volatile int* abort_sm = reinterpret_cast<volatile int*>(ctrl_p + 16 * C::STAGES + 16);
+    const uint32_t bar_full = ctrl, bar_empty = ctrl + 8 * ROWS_MAX_STAGES, bar_done = ctrl + 16 * ROWS_MAX_STAGES;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl_p + 16 * ROWS_MAX_STAGES + 8);
+    volatile int* abort_sm = reinterpret_cast<volatile int*>(ctrl_p + 16 * ROWS_MAX_STAGES + 16);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const WaitCtx wc{g.status, abort_sm};
@@ -513,7 +511,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
 
     if (threadIdx.x == 0) {
         *abort_sm = 0;
-        for (int s = 0; s < C::STAGES; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(bar_full + 8 * s, 1);
             mbar_init(bar_empty + 8 * s, 1);
         }
@@ -523,7 +521,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
         tma_prefetch_desc(&maps.x);
     }
     if (warp == 1) {
-        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), C::TMEM);
+        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), tmem_cols);
         tmem_relinquish<1>();
     }
     tc_fence_before();
@@ -543,12 +541,12 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
 
     if (warp == 0) {  // whole warps, one elected thread: as in ffn_gemm_kernel
         auto load_w = [&](int kb, int s) {
-            const uint32_t sw = ring + s * C::STAGE, full = bar_full + 8 * s;
-            mbar_expect_tx(full, C::STAGE);
+            const uint32_t sw = ring + s * stage, full = bar_full + 8 * s;
+            mbar_expect_tx(full, stage);
             if (GATED) {
                 // gate rows that do not exist read up rows instead, up rows zeros: not stored
                 tma_load_2d(sw, &maps.w, full, kb * BK, tile * 64);
-                tma_load_2d(sw + C::W_BYTES / 2, &maps.w, full, kb * BK, g.cols + tile * 64);
+                tma_load_2d(sw + ROWS_W_BYTES / 2, &maps.w, full, kb * BK, g.cols + tile * 64);
             } else if (W_MN) {
                 tma_load_2d(sw, &maps.w, full, tile * 128, kb * BK);
                 tma_load_2d(sw + MN_BLOCK, &maps.w, full, tile * 128 + 64, kb * BK);
@@ -557,9 +555,9 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
             }
         };
         auto load_x = [&](int kb, int s) {
-            tma_load_2d(ring + s * C::STAGE + C::W_BYTES, &maps.x, bar_full + 8 * s, kb * BK, tok0);
+            tma_load_2d(ring + s * stage + ROWS_W_BYTES, &maps.x, bar_full + 8 * s, kb * BK, tok0);
         };
-        const int ahead = min(kb1 - kb0, C::STAGES);
+        const int ahead = min(kb1 - kb0, stages);
         if (elect_one()) {
             for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
         }
@@ -577,13 +575,13 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
                 load_w(kb, s);
                 load_x(kb, s);
             }
-            if (++s == C::STAGES) {
+            if (++s == stages) {
                 s = 0;
                 ph ^= 1;
             }
         }
     } else if (warp == 1) {
-        constexpr uint32_t idesc = umma_idesc(1, 1, 128, N) | (W_MN ? 1u << 15 : 0u);
+        const uint32_t idesc = umma_idesc(1, 1, 128, N) | (W_MN ? 1u << 15 : 0u);
         constexpr uint64_t w_step = W_MN ? 16 * 128 / 16 : 2;
         int s = 0;
         uint32_t ph = 0;
@@ -594,15 +592,15 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
                 break;
             }
             tc_fence_after();
-            const uint64_t da = W_MN ? desc_mn(ring + s * C::STAGE) : umma_desc_sw128(ring + s * C::STAGE);
-            const uint64_t db = umma_desc_sw128(ring + s * C::STAGE + C::W_BYTES);
+            const uint64_t da = W_MN ? desc_mn(ring + s * stage) : umma_desc_sw128(ring + s * stage);
+            const uint64_t db = umma_desc_sw128(ring + s * stage + ROWS_W_BYTES);
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < BK / UMMA_K; ++k)
                     umma_f16<1>(tmem, da + w_step * k, db + 2 * k, idesc, kb != kb0 || k != 0);
                 umma_commit<1>(bar_empty + 8 * s);
             }
-            if (++s == C::STAGES) {
+            if (++s == stages) {
                 s = 0;
                 ph ^= 1;
             }
@@ -705,7 +703,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
             while (globaltimer_ns() - t0 < 200000ull) {
             }
         }
-        tmem_dealloc<1>(tmem, C::TMEM);
+        tmem_dealloc<1>(tmem, tmem_cols);
     }
 }
 
@@ -869,52 +867,44 @@ static int products(const Spec* s, int count, void* gu, bool follows, cudaStream
     return t.pair == 2 ? launch<EPI, 2>(maps, g, follows, st) : launch<EPI, 1>(maps, g, follows, st);
 }
 
-template <int EPI, bool W_MN, int N>
-static int launch_rows(const RowsMaps& maps, const RowsArgs& g, int tiles, int S, bool follows, cudaStream_t st) {
-    const auto kernel = ffn_rows_kernel<EPI, W_MN, N>;
-    static bool done[64] = {false};
-    const int rc = allow_smem(kernel, RowsCfg<N>::SMEM_BYTES, done);
-    if (rc != DK_OK) return rc;
-    Launch l(dim3(tiles * S, (g.T + N - 1) / N), ROWS_THREADS, RowsCfg<N>::SMEM_BYTES, S, follows, st);
-    DK_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, maps, g));
-    return DK_OK;
-}
-
-static int rows_tokens(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256; }
-
 // out [T, cols] = x W^T for few rows. GATED: W = W13, out = h; DGATED: x = dy, out = dgu. W_MN: W is [K, cols].
 template <int EPI, bool W_MN>
 static int rows_product(const void* x, const void* W, void* out, int T, int cols, int K, void* gu, bool follows,
                         cudaStream_t st) {
+    const auto kernel = ffn_rows_kernel<EPI, W_MN>;
+    static bool done[64] = {false};
     int sms = 0;
-    int rc = sm_count(&sms);
+    int rc = allow_smem(kernel, rows_smem(256), done);
+    if (rc == DK_OK) rc = sm_count(&sms);
     if (rc != DK_OK) return rc;
     const bool gated = EPI == EPI_GATED;
-    const int N = rows_tokens(T);
+    // Tokens of a tile: all of them, or 64 where reading the weights again is cheap (up to 16 MB they come from L2) and the
+    // shorter epilogue and the larger number of CTAs are worth more (256 rows of 1536 x 2048: 21.4 us against 26.6;
+    // of 8192 x 3584: 80 against 66).
+    const size_t weights = static_cast<size_t>(gated ? 2 : 1) * cols * K * 2;
+    const int N = T > 64 && weights <= (16u << 20) ? 64 : std::min(256, (T + 15) / 16 * 16);
     RowsMaps maps;
     rc = operand_map(&maps.w, W, W_MN, gated ? 2 * cols : cols, K, gated ? 64 : 128);
     if (rc == DK_OK) rc = operand_map(&maps.x, x, false, T, K, N);
-    if (rc != DK_OK) return rc;
     RowsArgs g{};
+    if (rc == DK_OK) rc = device_status_ptr(&g.status);
+    if (rc != DK_OK) return rc;
+    g.N = N;
     g.T = T;
     g.cols = cols;
     g.num_kb = (K + BK - 1) / BK;
     g.out = static_cast<__nv_bfloat16*>(out);
     g.gu = static_cast<float*>(gu);
-    rc = device_status_ptr(&g.status);
-    if (rc != DK_OK) return rc;
-    const int tiles = (cols + (gated ? 64 : 128) - 1) / (gated ? 64 : 128);
-    // cut K while the CTAs still run all at once and each keeps a few K blocks
+    const int tiles = (cols + (gated ? 64 : 128) - 1) / (gated ? 64 : 128), token_tiles = (T + N - 1) / N;
+    // Cut K while the CTAs still run all at once and each keeps two K blocks. Powers of two only: the places they leave
+    // go to the next product's CTAs, which start loading weights there (48 rows of 8192 x 3584: 41.4 us, with every place
+    // taken 43.3).
     const int places = sms * (N <= 128 ? 2 : 1);
     int S = 1;
-    while (S < 8 && tiles * S * 2 * ((T + N - 1) / N) <= places && g.num_kb / (S * 2) >= 2) S *= 2;
-    switch (N) {
-        case 16: return launch_rows<EPI, W_MN, 16>(maps, g, tiles, S, follows, st);
-        case 32: return launch_rows<EPI, W_MN, 32>(maps, g, tiles, S, follows, st);
-        case 64: return launch_rows<EPI, W_MN, 64>(maps, g, tiles, S, follows, st);
-        case 128: return launch_rows<EPI, W_MN, 128>(maps, g, tiles, S, follows, st);
-        default: return launch_rows<EPI, W_MN, 256>(maps, g, tiles, S, follows, st);
-    }
+    while (S < 8 && tiles * token_tiles * S * 2 <= places && g.num_kb >= S * 4) S *= 2;
+    Launch l(dim3(tiles * S, token_tiles), ROWS_THREADS, rows_smem(N), S, follows, st);
+    DK_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, maps, g));
+    return DK_OK;
 }
 
 // Few rows: see ffn_rows_kernel.

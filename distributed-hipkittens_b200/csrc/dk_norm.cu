@@ -97,6 +97,17 @@ __device__ __forceinline__ size_t mx_atom_offset(int row, int group4, int KB) {
     return ((static_cast<size_t>(rb) * KB + group4) * 32 + r0) * 16 + r1 * 4;
 }
 
+// Scale words of the last 128-row block's rows that do not exist: 0.
+__device__ __forceinline__ void mx_clear_padding(uint8_t* atoms, int rows, int H) {
+    const int left = rows & 127, words = H / 128 * 128;
+    if (left == 0) return;
+    uint32_t* block = reinterpret_cast<uint32_t*>(atoms) + static_cast<size_t>(rows >> 7) * words;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < words; i += gridDim.x * blockDim.x) {
+        const int w = i & 127;  // word 4 * (row % 32) + row / 32 of an atom
+        if ((w >> 2) + 32 * (w & 3) >= left) block[i] = 0u;
+    }
+}
+
 struct NormOut {
     void* y;      // rows, or null with MX
     float* rstd;  // may be null
@@ -141,6 +152,7 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* __restrict__ weight,
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
         if (j * per_row + tid < nvec) w[j].load(weight + static_cast<size_t>(j * per_row + tid) * V);
+    if constexpr (MX) mx_clear_padding(out.atoms, rows, H);
     int which = 0;
     for (int row = first; row < rows; row += stride, which ^= 1) {
         Pack<T, V> r[VPT];
@@ -228,6 +240,7 @@ add_rms_norm_wide_kernel(const T* x, const T* residual, const W* __restrict__ we
                          const NormOut out) {
     __shared__ float part[2][32];
     constexpr int STEP = MX ? 32 : 1;  // consecutive elements of a thread
+    if constexpr (MX) mx_clear_padding(out.atoms, rows, H);
     int which = 0;
     for (int row = blockIdx.x; row < rows; row += gridDim.x, which ^= 1) {
         const size_t base = static_cast<size_t>(row) * H;
@@ -584,10 +597,6 @@ extern "C" int dk_add_rms_norm_mx(const void* x, const void* residual, const voi
     DK_REQUIRE((residual != nullptr) == (r_out != nullptr), "r_out goes with a residual, and a residual with r_out");
     DK_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(s_rows) | reinterpret_cast<uintptr_t>(sf_atoms)) & 15) == 0,
                "q, s_rows and sf_atoms must be 16-byte aligned");
-    // rows of the last 128-row block that do not exist get scale byte 0
-    if (T % 128 != 0)
-        DK_CUDA_OK(cudaMemsetAsync(static_cast<uint8_t*>(sf_atoms) + static_cast<size_t>(T / 128) * (H / 128) * 512, 0,
-                                   static_cast<size_t>(H / 128) * 512, static_cast<cudaStream_t>(stream)));
     return launch_norm<true>(x, residual, weight, x_is_f32, w_is_f32, T, H, eps, r_out,
                              NormOut{nullptr, nullptr, static_cast<uint8_t*>(q), static_cast<uint8_t*>(s_rows),
                                      static_cast<uint8_t*>(sf_atoms)},

@@ -409,6 +409,7 @@ py::object moe_layer_ep(py::object X, py::object logits, int k, py::object W13q,
 // a kernel takes a few microseconds, so attribute names are interned and types compared by identity.
 struct Torch {
     PyObject *tensor, *bf16, *f32, *u8, *raw_stream;
+    PyObject* empty_like;
     PyObject *s_is_contiguous, *s_is_cuda, *s_get_device, *s_shape, *s_data_ptr, *s_dtype, *s_new_empty;
     PyObject* kw_dtype;
     Torch() {
@@ -418,6 +419,7 @@ struct Torch {
         bf16 = keep(t.attr("bfloat16"));
         f32 = keep(t.attr("float32"));
         u8 = keep(t.attr("uint8"));
+        empty_like = keep(t.attr("empty_like"));
         raw_stream = keep(py::getattr(t.attr("_C"), "_cuda_getCurrentRawStream", py::none()));
         s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
         s_is_cuda = PyUnicode_InternFromString("is_cuda");
@@ -478,13 +480,27 @@ void want_dtype(const Dense& d, PyObject* dtype, const char* name, const char* w
     if (d.dtype != dtype) throw std::runtime_error(std::string(name) + ": expected dtype " + what);
 }
 
-// Uninitialised tensor on the device of `like`, and its address.
-py::object new_empty(const py::object& like, int64_t rows, int64_t cols, PyObject* dtype, void** ptr) {
+// Uninitialised tensors on the device of `like`, and their addresses.
+void* address_of(const py::object& o) {
+    return PyLong_AsVoidPtr(checked(PyObject_CallMethodNoArgs(o.ptr(), torch_api().s_data_ptr)).ptr());
+}
+py::object new_empty(const py::object& like, const py::tuple& shape, PyObject* dtype, void** ptr) {
     const Torch& t = torch_api();
-    py::object shape = cols < 0 ? py::object(py::make_tuple(rows)) : py::object(py::make_tuple(rows, cols));
     PyObject* args[3] = {like.ptr(), shape.ptr(), dtype};
     py::object o = checked(PyObject_VectorcallMethod(t.s_new_empty, args, 2, t.kw_dtype));
-    if (ptr != nullptr) *ptr = PyLong_AsVoidPtr(checked(PyObject_CallMethodNoArgs(o.ptr(), t.s_data_ptr)).ptr());
+    *ptr = address_of(o);
+    return o;
+}
+py::object new_empty(const py::object& like, int64_t n, PyObject* dtype, void** ptr) {
+    return new_empty(like, py::make_tuple(n), dtype, ptr);
+}
+py::object new_empty(const py::object& like, int64_t rows, int64_t cols, PyObject* dtype, void** ptr) {
+    return new_empty(like, py::make_tuple(rows, cols), dtype, ptr);
+}
+// of the type and shape of `like` too (the fastest of torch's ways to a tensor); never a torch.nn.Parameter
+py::object empty_like(const py::object& like, void** ptr) {
+    py::object o = checked(PyObject_CallOneArg(torch_api().empty_like, like.ptr()));
+    *ptr = address_of(o);
     return o;
 }
 void* stream_of(int device) {
@@ -540,7 +556,7 @@ py::object stream_out(const NormArgs& a, const py::object& X, const py::object& 
         if (inplace) throw std::runtime_error("inplace needs a Residual");
         return X;
     }
-    if (!inplace) return new_empty(X, a.T, a.H, a.x_dtype, ptr);
+    if (!inplace) return empty_like(X, ptr);
     *ptr = a.res.ptr;
     return Residual;
 }
@@ -550,8 +566,8 @@ py::tuple add_rms_norm(py::object X, py::object Residual, py::object Weight, flo
     const NormArgs a = norm_args(X, Residual, Weight, "X", "Residual");
     void *yp, *rp, *sp;
     py::object r = stream_out(a, X, Residual, inplace, &rp);
-    py::object y = new_empty(X, a.T, a.H, a.x_dtype, &yp);
-    py::object rstd = new_empty(X, a.T, -1, t.f32, &sp);
+    py::object y = empty_like(X, &yp);
+    py::object rstd = new_empty(X, a.T, t.f32, &sp);
     throw_on(dk_add_rms_norm(a.x.ptr, a.res.ptr, a.w.ptr, a.x_f32, a.w_f32, a.T, a.H, eps, yp, rp,
                              static_cast<float*>(sp), stream_of(a.device)), "add_rms_norm");
     return py::make_tuple(y, r, rstd);
@@ -566,10 +582,10 @@ py::tuple add_rms_norm_mx(py::object X, py::object Residual, py::object Weight, 
     py::object q = new_empty(X, a.T, a.H, t.u8, &qp);
     py::object s = new_empty(X, a.T, a.H / 32, t.u8, &sp);
     const int64_t blocks = (static_cast<int64_t>(a.T) + 127) / 128;
-    py::object flat = new_empty(X, blocks * (a.H / 128), 512, t.u8, &ap);
+    py::object atoms = new_empty(X, py::make_tuple(blocks, a.H / 128, 512), t.u8, &ap);
     throw_on(dk_add_rms_norm_mx(a.x.ptr, a.res.ptr, a.w.ptr, a.x_f32, a.w_f32, a.T, a.H, eps, qp, sp, ap, rp,
                                 stream_of(a.device)), "add_rms_norm_mx");
-    return py::make_tuple(q, s, flat.attr("view")(blocks, a.H / 128, 512), r);
+    return py::make_tuple(q, s, atoms, r);
 }
 
 py::tuple add_rms_norm_bwd(py::object dY, py::object dR, py::object R, py::object rstd, py::object Weight) {
@@ -582,9 +598,9 @@ py::tuple add_rms_norm_bwd(py::object dY, py::object dR, py::object R, py::objec
     want_dtype(rs, t.f32, "rstd", "torch.float32");
     const size_t wb = dk_add_rms_norm_bwd_workspace_bytes(a.T, a.H);
     void *dxp, *dwp, *wsp;
-    py::object dx = new_empty(R, a.T, a.H, a.x_dtype, &dxp);
-    py::object dw = new_empty(R, a.H, -1, a.w_dtype, &dwp);
-    py::object ws = new_empty(R, static_cast<int64_t>(wb / 4), -1, t.f32, &wsp);
+    py::object dx = empty_like(R, &dxp);
+    py::object dw = empty_like(Weight, &dwp);
+    py::object ws = new_empty(R, static_cast<int64_t>(wb / 4), t.f32, &wsp);
     throw_on(dk_add_rms_norm_bwd(dy.ptr, a.res.ptr, a.x.ptr, static_cast<const float*>(rs.ptr), a.w.ptr, a.x_f32, a.w_f32,
                                  a.T, a.H, dxp, dwp, wsp, wb, stream_of(a.device)), "add_rms_norm_bwd");
     return py::make_tuple(dx, dw);
@@ -620,7 +636,7 @@ py::object gated_ffn(py::object X, py::object W13, py::object W2, bool save) {
     py::object gu;
     if (save) gu = new_empty(X, a.T, 2 * static_cast<int64_t>(a.F), torch_api().f32, &gup);
     py::object h = new_empty(X, a.T, a.F, bf16, &hp);
-    py::object y = new_empty(X, a.T, a.H, bf16, &yp);
+    py::object y = empty_like(X, &yp);
     throw_on(dk_gated_ffn(a.x.ptr, a.w13.ptr, a.w2.ptr, a.T, a.H, a.F, gup, hp, yp, stream_of(a.device)), "gated_ffn");
     if (save) return py::make_tuple(y, gu, h);
     return y;
@@ -637,9 +653,9 @@ py::tuple gated_ffn_bwd(py::object dY, py::object X, py::object W13, py::object 
         throw std::runtime_error("expected dY [T,H], GU [T,2F], H [T,F]");
     void *dgup, *dxp, *dw13p, *dw2p;
     py::object dgu = new_empty(X, a.T, F2, a.x.dtype, &dgup);
-    py::object dx = new_empty(X, a.T, a.H, a.x.dtype, &dxp);
-    py::object dw13 = new_empty(X, F2, a.H, a.x.dtype, &dw13p);
-    py::object dw2 = new_empty(X, a.H, a.F, a.x.dtype, &dw2p);
+    py::object dx = empty_like(X, &dxp);
+    py::object dw13 = empty_like(W13, &dw13p);
+    py::object dw2 = empty_like(W2, &dw2p);
     throw_on(dk_gated_ffn_bwd(dy.ptr, a.x.ptr, a.w13.ptr, a.w2.ptr, gu.ptr, h.ptr, a.T, a.H, a.F, dgup, dxp, dw13p, dw2p,
                               stream_of(a.device)), "gated_ffn_bwd");
     return py::make_tuple(dx, dw13, dw2);
