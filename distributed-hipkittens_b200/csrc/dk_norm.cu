@@ -17,6 +17,7 @@
 #include "dk_host.h"
 #include "dk_ptx.cuh"
 
+#include <algorithm>
 #include <initializer_list>
 
 namespace dk {
@@ -68,20 +69,113 @@ struct Pack {
     }
 };
 
-// Sum over the threads that share a row (a warp, or the CTA), the same value in every one of them and in
-// the same order on every run. `part` is used in turn by consecutive calls (which = 0, 1, 0, ...), so that one
-// barrier a call is enough: between two uses of a half lies the barrier of the other.
+// a + b, rounded once. Pairs of bf16 are added as such: the fp32 sum of two bf16 values, rounded to bf16, is the same
+// (what fp32 cannot hold of the smaller one lies below a 2^-8 part of the last place of bf16).
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> added(const Pack<T, V>& a, const Pack<T, V>& b) {
+    Pack<T, V> r;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+            reinterpret_cast<__nv_bfloat162*>(r.e)[i] =
+                __hadd2(reinterpret_cast<const __nv_bfloat162*>(a.e)[i], reinterpret_cast<const __nv_bfloat162*>(b.e)[i]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) r.e[k] = from_f32<T>(to_f32(a.e[k]) + to_f32(b.e[k]));
+    }
+    return r;
+}
+
+// Sum over the threads that share a row (a warp, or the first `threads` of the CTA), the same value in every one of
+// them and in the same order on every run. `part` is used in turn by consecutive calls (which = 0, 1, 0, ...), so that
+// one barrier a call is enough: between two uses of a half lies the barrier of the other.
 template <bool WARP>
-__device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int which) {
+__device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int which, int threads) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if constexpr (WARP) return v;
     if ((threadIdx.x & 31) == 0) part[which][threadIdx.x >> 5] = v;
-    __syncthreads();
+    named_bar_sync(1, threads);
     float s = 0.f;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) s += part[which][w];
+    for (int w = 0; w < (threads >> 5); ++w) s += part[which][w];
     return s;
 }
+
+// How the values of a row reach the threads of a backward pass.
+//   FROM_REGS   each thread loads its own 16-byte vectors (or elements), those of the next row as soon as it has added
+//               up this row's: they are in flight during the reduction and the writing
+//   FROM_WARP   the same, a row to a warp: no barrier
+//   FROM_RING   one thread has whole rows copied into a ring in shared memory (cp.async.bulk), as many rows ahead as
+//               fit: up to 200 KB in flight on an SM instead of what registers hold (8192 rows of 7168: 97 -> 80 us)
+// The forward pass stays with registers and two CTAs an SM: half the arrays and more arithmetic after the reduction, so
+// more warps are worth more than bytes in flight (a ring took 203 us instead of 182 for 16384 rows of 8192 with two CTAs,
+// 181 with one; 311 and 402 instead of 302 for 32768 rows of 7168 to MXFP8).
+enum : int { FROM_REGS = 0, FROM_WARP = 1, FROM_RING = 2 };
+constexpr int RING_STAGES = 12;
+constexpr int RING_SM_BYTES = 200 * 1024;  // rings of all CTAs of an SM
+enum : unsigned { SITE_NORM_ROW = 121 };
+struct Ring {
+    int stages, stage_bytes;  // a stage: the CTA's row of each array
+    unsigned* status;
+};
+struct RingShared {
+    uint64_t full[RING_STAGES];
+    int abort;
+};
+// The CTA's rows first, first + stride, ... of `n` arrays, a stage each. There is no barrier for empty stages: a thread
+// takes all it needs of a row into registers before the row's reduction, and the reduction's barrier then frees the stage.
+template <typename T, int N>
+struct RowRing {
+    RingShared& sh;
+    const Ring ring;
+    uint8_t* smem;
+    const T* const (&src)[N];
+    int n, stride, rows, H;
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void copy(int s, int row) {  // one thread
+        const uint32_t full = smem_u32(&sh.full[s]), bytes = static_cast<uint32_t>(H) * sizeof(T);
+        mbar_expect_tx(full, n * bytes);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < n)
+                bulk_load_1d(smem_u32(smem) + s * ring.stage_bytes + i * bytes, src[i] + static_cast<size_t>(row) * H, bytes,
+                             full);
+    }
+    __device__ __forceinline__ void start(int first) {
+        if (threadIdx.x == 0) {
+            sh.abort = 0;
+            for (int i = 0; i < ring.stages; ++i) mbar_init(smem_u32(&sh.full[i]), 1);
+            fence_mbar_init();
+            for (int i = 0; i < ring.stages && first + static_cast<int64_t>(i) * stride < rows; ++i) copy(i, first + i * stride);
+        }
+        __syncthreads();
+    }
+    // The row is there. A wait that gives up is recorded and the loop goes on: every thread still takes part in every
+    // barrier, the result is void.
+    __device__ __forceinline__ const T* wait(int row) {
+        const WaitCtx wc{ring.status, &sh.abort};
+        mbar_wait(smem_u32(&sh.full[stage]), phase, wc, SITE_NORM_ROW, row);
+        return reinterpret_cast<const T*>(smem + stage * ring.stage_bytes);
+    }
+    // A wait has given up: copies that are still in flight get time to land before the shared memory goes away.
+    __device__ __forceinline__ void finish() {
+        if (*static_cast<volatile int*>(&sh.abort)) {
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 200000ull) {
+            }
+        }
+    }
+    // After the row's reduction: the stage takes the row that is `stages` turns ahead.
+    __device__ __forceinline__ void next(int row) {
+        const int64_t ahead = row + static_cast<int64_t>(ring.stages) * stride;
+        if (threadIdx.x == 0 && ahead < rows) copy(stage, static_cast<int>(ahead));
+        if (++stage == ring.stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+};
 
 __device__ __forceinline__ float rstd_of(float sum_sq, int H, float eps) {
     return 1.0f / sqrtf(sum_sq / static_cast<float>(H) + eps);
@@ -98,11 +192,11 @@ __device__ __forceinline__ size_t mx_atom_offset(int row, int group4, int KB) {
 }
 
 // Scale words of the last 128-row block's rows that do not exist: 0.
-__device__ __forceinline__ void mx_clear_padding(uint8_t* atoms, int rows, int H) {
+__device__ __forceinline__ void mx_clear_padding(uint8_t* atoms, int rows, int H, int threads) {
     const int left = rows & 127, words = H / 128 * 128;
     if (left == 0) return;
     uint32_t* block = reinterpret_cast<uint32_t*>(atoms) + static_cast<size_t>(rows >> 7) * words;
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < words; i += gridDim.x * blockDim.x) {
+    for (int i = blockIdx.x * threads + threadIdx.x; i < words; i += gridDim.x * threads) {
         const int w = i & 127;  // word 4 * (row % 32) + row / 32 of an atom
         if ((w >> 2) + 32 * (w & 3) >= left) block[i] = 0u;
     }
@@ -115,15 +209,15 @@ struct NormOut {
 };
 
 // Rows that fit into registers: VPT vectors of V elements a thread, a row to a CTA (or to a warp where rows are
-// narrow). CTAs are persistent: the weight is read once, and the next row's loads are issued as soon as this
-// row's values have been added up, so that they are in flight during the reduction and the writing of y. Every
-// element is read once and written once.
+// narrow). CTAs are persistent: the weight is read once, and the next row's loads are issued as soon as this row's values
+// have been added up, so that they are in flight during the reduction and the writing of y. Every element is read once
+// and written once. NT: most threads that share a row.
 template <typename T, typename W, int V, int VPT, int NT, bool WARP, bool MX>
 __global__ void __launch_bounds__(NT)
 add_rms_norm_kernel(const T* x, const T* residual, const W* __restrict__ weight, int rows, int H, float eps, T* r_out,
                     const NormOut out) {
     __shared__ float part[2][32];
-    const int per_row = WARP ? 32 : blockDim.x;                       // threads of a row
+    const int per_row = WARP ? 32 : blockDim.x;  // threads of a row
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     const int stride = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
@@ -152,21 +246,17 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* __restrict__ weight,
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
         if (j * per_row + tid < nvec) w[j].load(weight + static_cast<size_t>(j * per_row + tid) * V);
-    if constexpr (MX) mx_clear_padding(out.atoms, rows, H);
+    if constexpr (MX) mx_clear_padding(out.atoms, rows, H, WARP ? blockDim.x : per_row);
     int which = 0;
     for (int row = first; row < rows; row += stride, which ^= 1) {
         Pack<T, V> r[VPT];
         float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            r[j] = a[j];
+            r[j] = residual != nullptr ? added(a[j], b[j]) : a[j];
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                float v = to_f32(a[j].e[k]);
-                if (residual != nullptr) {
-                    r[j].e[k] = from_f32<T>(v + to_f32(b[j].e[k]));
-                    v = to_f32(r[j].e[k]);
-                }
+                const float v = to_f32(r[j].e[k]);
                 ss += v * v;
             }
         }
@@ -177,7 +267,7 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* __restrict__ weight,
             for (int j = 0; j < VPT; ++j)
                 if (j * per_row + tid < nvec) r[j].store(r_out + base + static_cast<size_t>(j * per_row + tid) * V);
         }
-        const float rstd = rstd_of(row_sum<WARP>(ss, part, which), H, eps);
+        const float rstd = rstd_of(row_sum<WARP>(ss, part, which, per_row), H, eps);
         if (out.rstd != nullptr && tid == 0) out.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
@@ -196,18 +286,24 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* __restrict__ weight,
                 float f[V], amax = 0.f;
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    f[k] = to_f32(r[j].e[k]) * rstd * to_f32(w[j].e[k]);
+                    f[k] = to_f32(r[j].e[k]) * to_f32(w[j].e[k]);
                     amax = fmaxf(amax, fabsf(f[k]));
                 }
 #pragma unroll
                 for (int o = 1; o < BLOCK; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                const int e = mx_scale(amax);
-                const float inv = mx_inverse(e);
-                uint32_t word = 0;
-                const int lane = threadIdx.x & 31, lead = lane & ~(WORD - 1);
+                const int e = mx_scale(amax * rstd);
+                // y * 2^(127 - e) with one product: rstd times a power of two is exact while it stays clear of the ends of
+                // fp32 (rstd lies between 2^-64 and 2^64); outside, and for blocks of zeros, with two
+                float inv = rstd * mx_inverse(e);
+                if (e < 96 || e > 158) {
+                    inv = mx_inverse(e);
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    word |= static_cast<uint32_t>(__shfl_sync(0xffffffffu, e, lead + g * BLOCK)) << (8 * g);
+                    for (int k = 0; k < V; ++k) f[k] *= rstd;
+                }
+                uint32_t word = e;  // of the first lane of four blocks
+                word |= __shfl_down_sync(0xffffffffu, word, BLOCK) << 8;
+                word |= __shfl_down_sync(0xffffffffu, word, 2 * BLOCK) << 16;
+                const int lane = threadIdx.x & 31, lead = lane & ~(WORD - 1);
                 if (i < nvec) {
                     uint32_t p[V / 4];
 #pragma unroll
@@ -240,7 +336,7 @@ add_rms_norm_wide_kernel(const T* x, const T* residual, const W* __restrict__ we
                          const NormOut out) {
     __shared__ float part[2][32];
     constexpr int STEP = MX ? 32 : 1;  // consecutive elements of a thread
-    if constexpr (MX) mx_clear_padding(out.atoms, rows, H);
+    if constexpr (MX) mx_clear_padding(out.atoms, rows, H, NORM_THREADS);
     int which = 0;
     for (int row = blockIdx.x; row < rows; row += gridDim.x, which ^= 1) {
         const size_t base = static_cast<size_t>(row) * H;
@@ -255,7 +351,7 @@ add_rms_norm_wide_kernel(const T* x, const T* residual, const W* __restrict__ we
                 }
                 ss += v * v;
             }
-        const float rstd = rstd_of(row_sum<false>(ss, part, which), H, eps);
+        const float rstd = rstd_of(row_sum<false>(ss, part, which, NORM_THREADS), H, eps);
         if (out.rstd != nullptr && threadIdx.x == 0) out.rstd[row] = rstd;
         const T* r = residual != nullptr ? r_out : x;
         for (int c = threadIdx.x * STEP; c < H; c += NORM_THREADS * STEP) {
@@ -278,35 +374,48 @@ add_rms_norm_wide_kernel(const T* x, const T* residual, const W* __restrict__ we
     }
 }
 
-// Backward pass on the same plan: the row's dy, r and dr in registers, the next row's on their way, and the
-// thread's columns of dw summed in registers over the CTA's rows. Each CTA leaves one row of `partial`
-// [gridDim.x][H]; every element is summed by one thread in row order: the same bits on every run.
-template <typename T, typename W, int V, int VPT, int NT, bool WARP>
+// Backward pass on the same plan, with the thread's columns of dw summed in registers over the CTA's rows. Each CTA
+// leaves one row of `partial` [gridDim.x][H]; every element is summed by one thread in row order: the same bits on
+// every run.
+template <typename T, typename W, int V, int VPT, int NT, int FROM>
 __global__ void __launch_bounds__(NT)
 add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, const T* __restrict__ r,
                         const float* __restrict__ rstd_in, const W* __restrict__ weight, int rows, int H,
-                        T* __restrict__ dx, float* __restrict__ partial) {
+                        T* __restrict__ dx, float* __restrict__ partial, const Ring ring) {
+    constexpr bool WARP = FROM == FROM_WARP, RING = FROM == FROM_RING;
     __shared__ float part[2][32];
     __shared__ float warp_dw[WARP ? NT / 32 : 1][WARP ? 32 * VPT * V : 1];
+    __shared__ RingShared sh;
+    extern __shared__ __align__(128) uint8_t rows_smem[];
     const int per_row = WARP ? 32 : blockDim.x;
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     const int stride = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
     const int nvec = H / V;
+    const T* const src[3] = {dy, r, dr};
+    RowRing<T, 3> in{sh, ring, rows_smem, src, dr != nullptr ? 3 : 2, stride, rows, H};
+    if constexpr (RING) in.start(first);
     Pack<W, V> w[VPT];
     Pack<T, V> a[VPT], b[VPT], c[VPT];
     float next_rstd = 0.f;
     float dw[VPT][V];
-    auto fetch = [&](int row) {
-        const size_t base = static_cast<size_t>(row) * H;
+    auto fetch = [&](const T* p, const T* q) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int i = j * per_row + tid;
             if (i < nvec) {
-                a[j].load(dy + base + static_cast<size_t>(i) * V);
-                b[j].load(r + base + static_cast<size_t>(i) * V);
+                a[j].load(p + static_cast<size_t>(i) * V);
+                b[j].load(q + static_cast<size_t>(i) * V);
             }
         }
+    };
+    auto fetch_above = [&](const T* p) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+            if (j * per_row + tid < nvec) c[j].load(p + static_cast<size_t>(j * per_row + tid) * V);
+    };
+    auto fetch_row = [&](int row) {
+        fetch(dy + static_cast<size_t>(row) * H, r + static_cast<size_t>(row) * H);
         next_rstd = rstd_in[row];
     };
 #pragma unroll
@@ -318,7 +427,8 @@ add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, cons
 #pragma unroll
         for (int k = 0; k < V; ++k) dw[j][k] = 0.f;
     }
-    if (first < rows) fetch(first);
+    if (RING && first < rows) next_rstd = rstd_in[first];
+    if (!RING && first < rows) fetch_row(first);
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
         if (j * per_row + tid < nvec) w[j].load(weight + static_cast<size_t>(j * per_row + tid) * V);
@@ -326,10 +436,13 @@ add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, cons
     for (int row = first; row < rows; row += stride, which ^= 1) {
         const size_t base = static_cast<size_t>(row) * H;
         const float rstd = next_rstd;
-        if (dr != nullptr) {
-#pragma unroll
-            for (int j = 0; j < VPT; ++j)
-                if (j * per_row + tid < nvec) c[j].load(dr + base + static_cast<size_t>(j * per_row + tid) * V);
+        if constexpr (RING) {
+            if (row + stride < rows) next_rstd = rstd_in[row + stride];
+            const T* row_in = in.wait(row);
+            fetch(row_in, row_in + H);
+            if (dr != nullptr) fetch_above(row_in + 2 * H);
+        } else if (dr != nullptr) {
+            fetch_above(dr + base);
         }
         Pack<T, V> d[VPT], h[VPT];
         float dot = 0.f;
@@ -344,8 +457,9 @@ add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, cons
                 dw[j][k] += dn;
             }
         }
-        if (row + stride < rows) fetch(row + stride);
-        const float mean = row_sum<WARP>(dot, part, which) / static_cast<float>(H);
+        if (!RING && row + stride < rows) fetch_row(row + stride);
+        const float mean = row_sum<WARP>(dot, part, which, per_row) / static_cast<float>(H);
+        if constexpr (RING) in.next(row);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int i = j * per_row + tid;
@@ -362,6 +476,7 @@ add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, cons
             }
         }
     }
+    if constexpr (RING) in.finish();
     float* mine = partial + static_cast<size_t>(blockIdx.x) * H;
     if constexpr (WARP) {
 #pragma unroll
@@ -403,7 +518,7 @@ add_rms_norm_bwd_wide_kernel(const T* __restrict__ dy, const T* __restrict__ dr,
             dot += dn * to_f32(weight[c]);
             mine[c] += dn;
         }
-        const float mean = row_sum<false>(dot, part, which) / static_cast<float>(H);
+        const float mean = row_sum<false>(dot, part, which, NORM_THREADS) / static_cast<float>(H);
         for (int c = threadIdx.x; c < H; c += NORM_THREADS) {
             const float n = to_f32(r[base + c]) * rstd;
             float v = rstd * (to_f32(dy[base + c]) * to_f32(weight[c]) - n * mean);
@@ -441,8 +556,10 @@ add_rms_norm_dw_kernel(const float* __restrict__ partial, int parts, int H, W* _
 
 constexpr int NORM_MAX_H = 65536;
 constexpr int NORM_MAX_SMS = 160;
-// rows of `partial` at most: CTAs of a backward pass
-constexpr int NORM_BWD_PARTS = 2 * NORM_MAX_SMS;
+// CTAs of a backward pass on one SM at most, each with a row of `partial`: two, and for narrow rows as many as have
+// 32 KB of partial sums between them
+static int norm_bwd_ctas(int H) { return std::max(2, std::min(8, 8192 / H)); }
+static int norm_bwd_parts(int T, int H) { return std::min(T, NORM_MAX_SMS * norm_bwd_ctas(H)); }
 
 static int check_norm(const void* x, const void* weight, int x_is_f32, int w_is_f32, int T, int H) {
     DK_REQUIRE(T >= 0, "the number of rows must not be negative");
@@ -472,6 +589,30 @@ static NormPlan norm_plan(bool vec, int V, int T, int H, int sms) {
     if (!few && n <= 256) return NormPlan::ONE_WARP;
     if (n > 8192) return NormPlan::WIDE;
     return few ? NormPlan::ONE_FEW : NormPlan::ONE_MANY;
+}
+// Launch shape of a ring kernel: threads that share a row, CTAs on an SM and the ring of each.
+struct RingShape {
+    int threads, ctas, smem;
+    Ring ring;
+};
+static int ring_shape(int nvec, int H, int elem, int arrays, RingShape* out) {
+    const int threads = ((nvec + 3) / 4 + 31) / 32 * 32;
+    out->threads = threads;
+    out->ctas = std::max(1, 256 / threads);
+    out->ring.stage_bytes = arrays * H * elem;
+    out->ring.stages = std::max(2, std::min(RING_STAGES, RING_SM_BYTES / out->ctas / out->ring.stage_bytes));
+    out->smem = out->ring.stages * out->ring.stage_bytes;
+    return device_status_ptr(&out->ring.status);
+}
+template <typename K>
+static int allow_smem(K kernel, bool (&done)[64]) {
+    int dev = 0;
+    DK_CUDA_OK(cudaGetDevice(&dev));
+    if (!done[dev & 63]) {
+        DK_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_SM_BYTES));
+        done[dev & 63] = true;
+    }
+    return DK_OK;
 }
 static int round_threads(int n, int vpt) { return ((n + vpt - 1) / vpt + 31) / 32 * 32; }
 static bool aligned16(std::initializer_list<const void*> ps) {
@@ -522,7 +663,9 @@ static int launch_norm(const void* x, const void* residual, const void* weight, 
                     break;
                 }
             }
-            go(add_rms_norm_wide_kernel<T, W, MX>, NORM_THREADS, 1, 8);
+            add_rms_norm_wide_kernel<T, W, MX><<<rows < 8 * sms ? rows : 8 * sms, NORM_THREADS, 0, st>>>(
+                static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const W*>(weight), rows, H, eps,
+                static_cast<T*>(r_out), out);
     }
     DK_CUDA_OK(cudaGetLastError());
     return DK_OK;
@@ -547,22 +690,38 @@ static int launch_norm_bwd(const void* dy, const void* dr, const void* r, const 
     const NormPlan plan = norm_plan(vec, V, rows, H, sms);
     const int n = vec ? H / V : H;
     int parts = 0;
+    RingShape shape{};
+    auto grid = [&](int rows_per_cta, int ctas_per_sm) {
+        const int need = (rows + rows_per_cta - 1) / rows_per_cta, most = sms * std::min(ctas_per_sm, norm_bwd_ctas(H));
+        return parts = need < most ? need : most;
+    };
     auto go = [&](auto kernel, int threads, int rows_per_cta, int ctas_per_sm) {
-        const int need = (rows + rows_per_cta - 1) / rows_per_cta, most = sms * (ctas_per_sm < 2 ? ctas_per_sm : 2);
-        parts = need < most ? need : most;
-        kernel<<<parts, threads, 0, st>>>(static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r),
-                                          rstd, static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial);
+        kernel<<<grid(rows_per_cta, ctas_per_sm), threads, shape.smem, st>>>(
+            static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r), rstd,
+            static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial, shape.ring);
     };
     switch (plan) {
-        case NormPlan::VEC_FEW: go(add_rms_norm_bwd_kernel<T, W, V, 1, 1024, false>, round_threads(n, 1), 1, 1); break;
-        case NormPlan::VEC_FEW2: go(add_rms_norm_bwd_kernel<T, W, V, 2, 1024, false>, round_threads(n, 2), 1, 1); break;
-        case NormPlan::VEC_MANY: go(add_rms_norm_bwd_kernel<T, W, V, 4, 256, false>, round_threads(n, 4), 1, 1); break;
-        case NormPlan::VEC_MANY512: go(add_rms_norm_bwd_kernel<T, W, V, 4, 512, false>, round_threads(n, 4), 1, 1); break;
-        case NormPlan::VEC_WARP: go(add_rms_norm_bwd_kernel<T, W, V, 4, 256, true>, 256, 8, 2); break;
-        case NormPlan::ONE_FEW: go(add_rms_norm_bwd_kernel<T, W, 1, 8, 1024, false>, round_threads(n, 8), 1, 1); break;
-        case NormPlan::ONE_MANY: go(add_rms_norm_bwd_kernel<T, W, 1, 16, 512, false>, round_threads(n, 16), 1, 2); break;
-        case NormPlan::ONE_WARP: go(add_rms_norm_bwd_kernel<T, W, 1, 8, 256, true>, 256, 8, 2); break;
-        case NormPlan::WIDE: go(add_rms_norm_bwd_wide_kernel<T, W>, NORM_THREADS, 1, 2); break;
+        case NormPlan::VEC_FEW: go(add_rms_norm_bwd_kernel<T, W, V, 1, 1024, FROM_REGS>, round_threads(n, 1), 1, 1); break;
+        case NormPlan::VEC_FEW2: go(add_rms_norm_bwd_kernel<T, W, V, 2, 1024, FROM_REGS>, round_threads(n, 2), 1, 1); break;
+        case NormPlan::VEC_MANY: {
+            const auto kernel = add_rms_norm_bwd_kernel<T, W, V, 4, 256, FROM_RING>;
+            static bool done[64] = {false};
+            int rc2 = allow_smem(kernel, done);
+            if (rc2 == DK_OK) rc2 = ring_shape(n, H, sizeof(T), dr != nullptr ? 3 : 2, &shape);
+            if (rc2 != DK_OK) return rc2;
+            go(kernel, shape.threads, 1, shape.ctas);
+            break;
+        }
+        case NormPlan::VEC_MANY512: go(add_rms_norm_bwd_kernel<T, W, V, 4, 512, FROM_REGS>, round_threads(n, 4), 1, 1); break;
+        case NormPlan::VEC_WARP: go(add_rms_norm_bwd_kernel<T, W, V, 4, 256, FROM_WARP>, 256, 8, 2); break;
+        case NormPlan::ONE_FEW: go(add_rms_norm_bwd_kernel<T, W, 1, 8, 1024, FROM_REGS>, round_threads(n, 8), 1, 1); break;
+        case NormPlan::ONE_MANY: go(add_rms_norm_bwd_kernel<T, W, 1, 16, 512, FROM_REGS>, round_threads(n, 16), 1, 2); break;
+        case NormPlan::ONE_WARP: go(add_rms_norm_bwd_kernel<T, W, 1, 8, 256, FROM_WARP>, 256, 8, 2); break;
+        case NormPlan::WIDE:
+            add_rms_norm_bwd_wide_kernel<T, W><<<grid(1, 2), NORM_THREADS, 0, st>>>(
+                static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r), rstd,
+                static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial);
+            break;
     }
     DK_CUDA_OK(cudaGetLastError());
     add_rms_norm_dw_kernel<W><<<(H + 31) / 32, 256, 0, st>>>(partial, parts, H, static_cast<W*>(dw));
@@ -606,7 +765,7 @@ extern "C" int dk_add_rms_norm_mx(const void* x, const void* residual, const voi
 extern "C" size_t dk_add_rms_norm_bwd_workspace_bytes(int T, int H) {
     using namespace dk;
     if (T < 0 || H < 1 || H > NORM_MAX_H) return 0;
-    return static_cast<size_t>(T < NORM_BWD_PARTS ? T : NORM_BWD_PARTS) * H * sizeof(float);
+    return static_cast<size_t>(norm_bwd_parts(T, H)) * H * sizeof(float);
 }
 
 extern "C" int dk_add_rms_norm_bwd(const void* dy, const void* dr, const void* r, const float* rstd, const void* weight,
