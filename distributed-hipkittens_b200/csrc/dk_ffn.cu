@@ -62,7 +62,7 @@ enum : unsigned { SITE_EMPTY = 101, SITE_FULL = 102, SITE_TMEM_EMPTY = 103, SITE
 constexpr int MAX_PRODUCTS = 3;
 struct Maps {
     CUtensorMap a[MAX_PRODUCTS], b[MAX_PRODUCTS];
-    CUtensorMap out[MAX_PRODUCTS];  // STORE: D of each product; GATED: h, g, u; DGATED: dg, du
+    CUtensorMap out[MAX_PRODUCTS];  // STORE: D of each product; GATED: h, g, u
 };
 
 struct Product {
@@ -76,7 +76,8 @@ struct Args {
     int products, num_tiles;
     int bn;           // width of the B tile (GATED: gate and up rows together)
     int save;         // GATED: g and u leave too
-    const float* gu;  // DGATED: kept [g|u], [M, 2N]
+    const float* gu;     // DGATED: kept [g|u], [M, 2N]
+    __nv_bfloat16* dgu;  // DGATED: [dg|du], [M, 2N]
     unsigned* status;
 };
 
@@ -339,6 +340,14 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
             rows = g.p[pi].M;
             cols = g.p[pi].N;
             const int row0 = (m * PAIR + crank) * BM + q * 32;
+            float next_gate[32], next_up[32];  // DGATED
+            auto kept = [&](size_t place, int col) {
+                const bool ok = row0 + lane < rows;
+                ld_row32(g.gu + place, col, cols, ok, next_gate);
+                ld_row32(g.gu + place + cols, col, cols, ok, next_up);
+            };
+            if constexpr (EPI == EPI_DGATED)
+                kept(static_cast<size_t>(row0 + lane) * (2 * static_cast<size_t>(cols)) + n * bn, n * bn);
             if (!__all_sync(0xffffffffu, mbar_wait(bar_tfull + 8 * acc, acc_ph, wc, SITE_TMEM_FULL, t))) break;
             tc_fence_after();
             const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN_MAX;
@@ -393,33 +402,37 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
                     send(buf, &maps.out[0], col, row0);
                 }
             } else {
-                const int row = row0 + lane;
-                const bool row_ok = row < rows;
-                const float* gu = g.gu + static_cast<size_t>(row) * (2 * static_cast<size_t>(cols));
+                // A lane's 64 bytes of dg and of du leave from registers, whole sectors each; the g and u of the next
+                // 32 columns are on their way meanwhile.
+                const size_t at = static_cast<size_t>(row0 + lane) * (2 * static_cast<size_t>(cols)) + n * bn;
+                __nv_bfloat16* const dg_row = g.dgu + at;
+                const int units = bn / 32;
 #pragma unroll 1
-                for (int c = 0; c < bn / 64; ++c) {
-                    const int col0 = n * bn + c * 64;
-                    const uint32_t bg = next_buf();
-                    uint32_t pu[2][16];
+                for (int c = 0; c < units; ++c) {
+                    const int col = n * bn + c * 32;
+                    float gate[32], up[32], dh[32];
 #pragma unroll
-                    for (int hi = 0; hi < 2; ++hi) {
-                        const int col = col0 + hi * 32;
-                        float gate[32], up[32], dh[32];
-                        ld_row32(gu + col, col, cols, row_ok, gate);
-                        ld_row32(gu + cols + col, col, cols, row_ok, up);
-                        ld_acc(t_acc + c * 64 + hi * 32, dh);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) d_gated(dh[i], gate[i], up[i], gate[i], dh[i]);
-                        uint32_t pg[16];
-                        pack32(gate, pg);
-                        stage_half(bg, lane, hi, pg);
-                        pack32(dh, pu[hi]);
+                    for (int i = 0; i < 32; ++i) {
+                        gate[i] = next_gate[i];
+                        up[i] = next_up[i];
                     }
-                    send(bg, &maps.out[0], col0, row0);
-                    const uint32_t bu = next_buf();
-                    stage_half(bu, lane, 0, pu[0]);
-                    stage_half(bu, lane, 1, pu[1]);
-                    send(bu, &maps.out[1], col0, row0);
+                    if (c + 1 < units) kept(at + (c + 1) * 32, col + 32);
+                    ld_acc(t_acc + c * 32, dh);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) d_gated(dh[i], gate[i], up[i], gate[i], dh[i]);
+                    uint32_t pg[16], pu[16];
+                    pack32(gate, pg);
+                    pack32(dh, pu);
+                    if (row0 + lane < rows) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (col + 8 * j >= cols) break;
+                            __nv_bfloat16* to = dg_row + c * 32 + 8 * j;
+                            *reinterpret_cast<uint4*>(to) = make_uint4(pg[4 * j], pg[4 * j + 1], pg[4 * j + 2], pg[4 * j + 3]);
+                            *reinterpret_cast<uint4*>(to + cols) =
+                                make_uint4(pu[4 * j], pu[4 * j + 1], pu[4 * j + 2], pu[4 * j + 3]);
+                        }
+                    }
                 }
             }
             tc_fence_before();
@@ -847,8 +860,7 @@ static int products(const Spec* s, int count, void* gu, bool follows, cudaStream
         };
         const uint64_t n = static_cast<uint64_t>(p.N);
         if (EPI == EPI_DGATED) {
-            out(0, s[i].D, 4 * n, 1);
-            out(1, static_cast<__nv_bfloat16*>(s[i].D) + n, 4 * n, 1);
+            g.dgu = static_cast<__nv_bfloat16*>(s[i].D);
         } else {
             out(i, s[i].D, 2 * n, 1);
             if (EPI == EPI_GATED && gu != nullptr) {

@@ -392,6 +392,7 @@ add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, cons
     const int first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     const int stride = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
     const int nvec = H / V;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const T* const src[3] = {dy, r, dr};
     RowRing<T, 3> in{sh, ring, rows_smem, src, dr != nullptr ? 3 : 2, stride, rows, H};
     if constexpr (RING) in.start(first);
@@ -506,6 +507,7 @@ add_rms_norm_bwd_wide_kernel(const T* __restrict__ dy, const T* __restrict__ dr,
                              const float* __restrict__ rstd_in, const W* __restrict__ weight, int rows, int H,
                              T* __restrict__ dx, float* __restrict__ partial) {
     __shared__ float part[2][32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     float* mine = partial + static_cast<size_t>(blockIdx.x) * H;
     for (int c = threadIdx.x; c < H; c += NORM_THREADS) mine[c] = 0.f;
     int which = 0;
@@ -529,16 +531,18 @@ add_rms_norm_bwd_wide_kernel(const T* __restrict__ dy, const T* __restrict__ dr,
 }
 
 // dw[c] = sum of the CTAs' partial sums: 32 columns to a CTA, its eight warps each take every eighth part, and
-// their sums are added up in order.
+// their sums are added up in order. Launched while the backward pass still runs (its CTAs fit beside that one's), it
+// waits for its end on the device.
 template <typename W>
 __global__ void __launch_bounds__(256)
 add_rms_norm_dw_kernel(const float* __restrict__ partial, int parts, int H, W* __restrict__ dw) {
     __shared__ float sum[8][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     float s = 0.f;
     if (c < H) {
-#pragma unroll 4
+#pragma unroll 16
         for (int p = warp; p < parts; p += 8) s += partial[static_cast<size_t>(p) * H + c];
     }
     sum[warp][lane] = s;
@@ -724,8 +728,17 @@ static int launch_norm_bwd(const void* dy, const void* dr, const void* r, const 
             break;
     }
     DK_CUDA_OK(cudaGetLastError());
-    add_rms_norm_dw_kernel<W><<<(H + 31) / 32, 256, 0, st>>>(partial, parts, H, static_cast<W*>(dw));
-    DK_CUDA_OK(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((H + 31) / 32);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    DK_CUDA_OK(cudaLaunchKernelEx(&cfg, add_rms_norm_dw_kernel<W>, static_cast<const float*>(partial), parts, H,
+                                  static_cast<W*>(dw)));
     return DK_OK;
 }
 
