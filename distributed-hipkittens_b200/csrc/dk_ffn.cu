@@ -33,6 +33,7 @@
 // leader's barrier, the leader issues the MMAs. PAIR = 1: one CTA per 128x256 tile, for row counts whose last pair
 // would be half empty.
 #include "dk_host.h"
+#include "dk_launch.cuh"
 #include "dk_ptx.cuh"
 
 #include <algorithm>
@@ -146,7 +147,7 @@ __device__ __forceinline__ void ld_row32(const float* p, int col, int n, bool ok
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (ok && col + 4 * j < n) v = __ldg(reinterpret_cast<const float4*>(p) + j);
+        if (ok && col + 4 * j < n) v = reinterpret_cast<const float4*>(p)[j];
         f[4 * j] = v.x;
         f[4 * j + 1] = v.y;
         f[4 * j + 2] = v.z;
@@ -204,16 +205,14 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
     }
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    // a kernel of the same call that follows may take the places this one's CTAs leave; this one, when it follows,
-    // reads nothing before the one before it is complete (everything else hangs on the producer's loads)
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    next_may_begin();
+    previous_done();
 
     // Producer and issuer run their loops as whole warps and elect one thread for the instructions themselves: what
     // the instructions take (descriptors, coordinates, barriers) then stays in uniform registers. With one thread
     // in the loops a stage of 64 of K took 0.37 us to issue whatever its width; now 0.27 (128 columns).
     if (warp == 0) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        asm volatile("fence.proxy.async;" ::: "memory");
+        asm volatile("fence.proxy.async;" ::: "memory");  // what earlier kernels wrote, for the copy engine
         const int b_rows = bn / PAIR;
         const uint32_t tx = A_BYTES + b_rows * BK * 2;
         int s = 0;
@@ -474,12 +473,13 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
 //   EPI_GATED   a tile is 64 gate rows and the 64 up rows of the same columns; silu(g) * u leaves as h
 //   EPI_STORE   y from h and W2, or dx from [dg|du] and W13 (MN-major: 128 columns of W13)
 //   EPI_DGATED  dh from dy and W2 (MN-major: 128 columns of W2), with the kept g, u straight into dg, du
-// A product that follows another of the same call may start while that one still runs: its weights do not depend
-// on it, so the ring is filled with them, and only then does it wait for the rows it reads.
+// Half of the time of a small product is its beginning and its end, when HBM is idle; see the producer for what it does
+// meanwhile.
 constexpr int ROWS_THREADS = 192;
 constexpr int ROWS_W_BYTES = 128 * BK * 2;
 // Shared memory of the ring: two CTAs on an SM up to 128 tokens, one above. The partial sums reuse it: N * 512 bytes.
 constexpr int ROWS_MAX_STAGES = 8;
+constexpr int64_t ROWS_PREFETCH = 32 << 20;  // bytes of weights that go to L2 ahead: what HBM delivers in 5 us
 __host__ __device__ constexpr int rows_ring(int N) { return N <= 128 ? 110 * 1024 : 208 * 1024; }
 constexpr int rows_smem(int N) { return 1024 + rows_ring(N) + 256; }
 static_assert(128 * 512 <= rows_ring(128) && 256 * 512 <= rows_ring(256), "the partial sums reuse the ring");
@@ -488,11 +488,18 @@ struct RowsMaps {
 };
 struct RowsArgs {
     int N;                // tokens of a tile, a multiple of 16
+    int weights_ready;    // the kernel before this one belongs to the same call
+    int prefetch;         // K blocks of weights that go to L2 ahead
     int T, cols, num_kb;  // cols: columns of the output (GATED, DGATED: F)
     __nv_bfloat16* out;   // [T, cols]; DGATED: [T, 2 cols]
     float* gu;            // [T, 2 cols]; GATED: written, may be null; DGATED: read
     unsigned* status;
 };
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* m, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x),
+                 "r"(y)
+                 : "memory");
+}
 __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
     float2 v;
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
@@ -550,7 +557,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
             cluster_wait();
         }
     };
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // as in ffn_gemm_kernel
+    next_may_begin();
 
     if (warp == 0) {  // whole warps, one elected thread: as in ffn_gemm_kernel
         auto load_w = [&](int kb, int s) {
@@ -572,13 +579,31 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
         };
         const int ahead = min(kb1 - kb0, stages);
         if (elect_one()) {
-            for (int i = 0; i < ahead; ++i) load_w(kb0 + i, i);
+            // While an earlier kernel still runs, its end being bound by a few CTAs, HBM is free. After a kernel of the same
+            // call, which writes no weights, the ring takes its first stages of them and L2 the next ones; otherwise L2 all.
+            const int first = g.weights_ready ? ahead : 0;
+            for (int i = 0; i < first; ++i) load_w(kb0 + i, i);
+            const int last = min(kb1, kb0 + first + g.prefetch);
+            for (int kb = kb0 + first; kb < last; ++kb) {
+                if (GATED) {
+                    tma_prefetch_2d(&maps.w, kb * BK, tile * 64);
+                    tma_prefetch_2d(&maps.w, kb * BK, g.cols + tile * 64);
+                } else if (W_MN) {
+                    tma_prefetch_2d(&maps.w, tile * 128, kb * BK);
+                    tma_prefetch_2d(&maps.w, tile * 128 + 64, kb * BK);
+                } else {
+                    tma_prefetch_2d(&maps.w, kb * BK, tile * 128);
+                }
+            }
         }
-        // what the kernel before wrote is complete and visible from here on, to the copy engine too
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        asm volatile("fence.proxy.async;" ::: "memory");
+        __syncwarp();
+        previous_done();
+        asm volatile("fence.proxy.async;" ::: "memory");  // what earlier kernels wrote, for the copy engine
         if (elect_one()) {
-            for (int i = 0; i < ahead; ++i) load_x(kb0 + i, i);
+            for (int i = 0; i < ahead; ++i) {
+                if (!g.weights_ready) load_w(kb0 + i, i);
+                load_x(kb0 + i, i);
+            }
         }
         int s = 0;
         uint32_t ph = 0;
@@ -639,6 +664,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
         }
     }
     tc_fence_before();
+    previous_done();  // for every thread that writes, or reads the kept g and u
     meet();
     {
         constexpr int PAIRS = GATED ? 32 : 64;  // pairs of neighbouring output columns of a tile
@@ -729,26 +755,6 @@ static int operand_map(CUtensorMap* map, const void* p, bool mn, int rows_or_col
     return make_tmap_2d(map, p, 2, K, rows_or_cols, static_cast<uint64_t>(K) * 2, BK, box);
 }
 
-// Launch attributes: the cluster's size, and (`follows`) the permission to start while the kernel before it on the
-// stream, which is one of the same call, still runs.
-struct Launch {
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[2];
-    Launch(dim3 grid, int threads, int smem, int cluster, bool follows, cudaStream_t st) {
-        cfg.gridDim = grid;
-        cfg.blockDim = dim3(threads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = st;
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = cluster;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[1].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = follows ? 2 : 1;
-    }
-};
 template <typename K>
 static int allow_smem(K kernel, int bytes, bool (&done)[64]) {
     int dev = 0;
@@ -761,7 +767,7 @@ static int allow_smem(K kernel, int bytes, bool (&done)[64]) {
 }
 
 template <int EPI, int PAIR>
-static int launch(const Maps& maps, const Args& g, bool follows, cudaStream_t st) {
+static int launch(const Maps& maps, const Args& g, cudaStream_t st) {
     const auto kernel = ffn_gemm_kernel<EPI, PAIR>;
     static bool done[64] = {false};
     int sms = 0;
@@ -769,9 +775,7 @@ static int launch(const Maps& maps, const Args& g, bool follows, cudaStream_t st
     if (rc == DK_OK) rc = sm_count(&sms);
     if (rc != DK_OK) return rc;
     const int units = sms / PAIR;
-    Launch l(dim3((g.num_tiles < units ? g.num_tiles : units) * PAIR), THREADS, SMEM_BYTES, PAIR, follows, st);
-    DK_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, maps, g));
-    return DK_OK;
+    return launch_early(kernel, dim3((g.num_tiles < units ? g.num_tiles : units) * PAIR), THREADS, SMEM_BYTES, PAIR, st, maps, g);
 }
 
 // One product: D[M,N] = A B. GATED: B = W13 [2N, K], D = h; DGATED: D = dgu [M, 2N].
@@ -827,7 +831,7 @@ static Tiling choose(const Spec* s, int count, int epi, int sms) {
 
 // gu: GATED: where g and u go (may be null); DGATED: where they come from
 template <int EPI>
-static int products(const Spec* s, int count, void* gu, bool follows, cudaStream_t st) {
+static int products(const Spec* s, int count, void* gu, cudaStream_t st) {
     int sms = 0;
     int rc = sm_count(&sms);
     if (rc != DK_OK) return rc;
@@ -876,7 +880,7 @@ static int products(const Spec* s, int count, void* gu, bool follows, cudaStream
     g.gu = static_cast<const float*>(gu);
     rc = device_status_ptr(&g.status);
     if (rc != DK_OK) return rc;
-    return t.pair == 2 ? launch<EPI, 2>(maps, g, follows, st) : launch<EPI, 1>(maps, g, follows, st);
+    return t.pair == 2 ? launch<EPI, 2>(maps, g, st) : launch<EPI, 1>(maps, g, st);
 }
 
 // out [T, cols] = x W^T for few rows. GATED: W = W13, out = h; DGATED: x = dy, out = dgu. W_MN: W is [K, cols].
@@ -914,9 +918,9 @@ static int rows_product(const void* x, const void* W, void* out, int T, int cols
     const int places = sms * (N <= 128 ? 2 : 1);
     int S = 1;
     while (S < 8 && tiles * token_tiles * S * 2 <= places && g.num_kb >= S * 4) S *= 2;
-    Launch l(dim3(tiles * S, token_tiles), ROWS_THREADS, rows_smem(N), S, follows, st);
-    DK_CUDA_OK(cudaLaunchKernelEx(&l.cfg, kernel, maps, g));
-    return DK_OK;
+    g.weights_ready = follows;
+    g.prefetch = static_cast<int>(std::min<int64_t>(g.num_kb, ROWS_PREFETCH / (static_cast<int64_t>(tiles) * S * ROWS_W_BYTES)));
+    return launch_early(kernel, dim3(tiles * S, token_tiles), ROWS_THREADS, rows_smem(N), S, st, maps, g);
 }
 
 // Few rows: see ffn_rows_kernel.
@@ -957,9 +961,9 @@ extern "C" int dk_gated_ffn(const void* x, const void* w13, const void* w2, int 
         return rows_product<EPI_STORE, false>(h, w2, y, T, H, F, nullptr, true, st);
     }
     const Spec up{x, w13, h, T, F, H, false, false}, down{h, w2, y, T, H, F, false, false};
-    rc = products<EPI_GATED>(&up, 1, gu, false, st);
+    rc = products<EPI_GATED>(&up, 1, gu, st);
     if (rc != DK_OK) return rc;
-    return products<EPI_STORE>(&down, 1, nullptr, true, st);
+    return products<EPI_STORE>(&down, 1, nullptr, st);
 }
 
 extern "C" int dk_gated_ffn_bwd(const void* dy, const void* x, const void* w13, const void* w2, const void* gu, const void* h,
@@ -985,11 +989,11 @@ extern "C" int dk_gated_ffn_bwd(const void* dy, const void* x, const void* w13, 
         rc = rows_product<EPI_DGATED, true>(dy, w2, dgu, T, F, H, const_cast<void*>(gu), false, st);
         if (rc == DK_OK) rc = rows_product<EPI_STORE, true>(dgu, w13, dx, T, H, 2 * F, nullptr, true, st);
         const Spec two[2] = {d_w13, d_w2};
-        if (rc == DK_OK) rc = products<EPI_STORE>(two, 2, nullptr, true, st);
+        if (rc == DK_OK) rc = products<EPI_STORE>(two, 2, nullptr, st);
         return rc;
     }
     const Spec d_h{dy, w2, dgu, T, F, H, false, true}, d_x{dgu, w13, dx, T, H, 2 * F, false, true};
-    rc = products<EPI_DGATED>(&d_h, 1, const_cast<void*>(gu), false, st);
+    rc = products<EPI_DGATED>(&d_h, 1, const_cast<void*>(gu), st);
     if (rc != DK_OK) return rc;
     // the longest tiles first
     Spec three[3] = {d_x, d_w13, d_w2};
@@ -998,6 +1002,6 @@ extern "C" int dk_gated_ffn_bwd(const void* dy, const void* x, const void* w13, 
         three[1] = d_w2;
         three[2] = d_x;
     }
-    rc = products<EPI_STORE>(three, 3, nullptr, true, st);
+    rc = products<EPI_STORE>(three, 3, nullptr, st);
     return rc;
 }

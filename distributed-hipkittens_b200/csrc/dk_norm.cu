@@ -15,6 +15,7 @@
 #include <cuda_fp8.h>
 
 #include "dk_host.h"
+#include "dk_launch.cuh"
 #include "dk_ptx.cuh"
 
 #include <algorithm>
@@ -214,9 +215,11 @@ struct NormOut {
 // and written once. NT: most threads that share a row.
 template <typename T, typename W, int V, int VPT, int NT, bool WARP, bool MX>
 __global__ void __launch_bounds__(NT)
-add_rms_norm_kernel(const T* x, const T* residual, const W* __restrict__ weight, int rows, int H, float eps, T* r_out,
+add_rms_norm_kernel(const T* x, const T* residual, const W* weight, int rows, int H, float eps, T* r_out,
                     const NormOut out) {
     __shared__ float part[2][32];
+    next_may_begin();
+    previous_done();
     const int per_row = WARP ? 32 : blockDim.x;  // threads of a row
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -332,10 +335,12 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* __restrict__ weight,
 // meets the same elements in both, so r_out may be the residual's or x's own buffer.
 template <typename T, typename W, bool MX>
 __global__ void __launch_bounds__(NORM_THREADS)
-add_rms_norm_wide_kernel(const T* x, const T* residual, const W* __restrict__ weight, int rows, int H, float eps, T* r_out,
+add_rms_norm_wide_kernel(const T* x, const T* residual, const W* weight, int rows, int H, float eps, T* r_out,
                          const NormOut out) {
     __shared__ float part[2][32];
     constexpr int STEP = MX ? 32 : 1;  // consecutive elements of a thread
+    next_may_begin();
+    previous_done();
     if constexpr (MX) mx_clear_padding(out.atoms, rows, H, NORM_THREADS);
     int which = 0;
     for (int row = blockIdx.x; row < rows; row += gridDim.x, which ^= 1) {
@@ -379,9 +384,9 @@ add_rms_norm_wide_kernel(const T* x, const T* residual, const W* __restrict__ we
 // every run.
 template <typename T, typename W, int V, int VPT, int NT, int FROM>
 __global__ void __launch_bounds__(NT)
-add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, const T* __restrict__ r,
-                        const float* __restrict__ rstd_in, const W* __restrict__ weight, int rows, int H,
-                        T* __restrict__ dx, float* __restrict__ partial, const Ring ring) {
+add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
+                        const float* rstd_in, const W* weight, int rows, int H,
+                        T* dx, float* partial, const Ring ring) {
     constexpr bool WARP = FROM == FROM_WARP, RING = FROM == FROM_RING;
     __shared__ float part[2][32];
     __shared__ float warp_dw[WARP ? NT / 32 : 1][WARP ? 32 * VPT * V : 1];
@@ -392,7 +397,8 @@ add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, cons
     const int first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     const int stride = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
     const int nvec = H / V;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    next_may_begin();
+    previous_done();
     const T* const src[3] = {dy, r, dr};
     RowRing<T, 3> in{sh, ring, rows_smem, src, dr != nullptr ? 3 : 2, stride, rows, H};
     if constexpr (RING) in.start(first);
@@ -503,11 +509,12 @@ add_rms_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dr, cons
 // Any width and alignment.
 template <typename T, typename W>
 __global__ void __launch_bounds__(NORM_THREADS)
-add_rms_norm_bwd_wide_kernel(const T* __restrict__ dy, const T* __restrict__ dr, const T* __restrict__ r,
-                             const float* __restrict__ rstd_in, const W* __restrict__ weight, int rows, int H,
-                             T* __restrict__ dx, float* __restrict__ partial) {
+add_rms_norm_bwd_wide_kernel(const T* dy, const T* dr, const T* r,
+                             const float* rstd_in, const W* weight, int rows, int H,
+                             T* dx, float* partial) {
     __shared__ float part[2][32];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    next_may_begin();
+    previous_done();
     float* mine = partial + static_cast<size_t>(blockIdx.x) * H;
     for (int c = threadIdx.x; c < H; c += NORM_THREADS) mine[c] = 0.f;
     int which = 0;
@@ -535,11 +542,12 @@ add_rms_norm_bwd_wide_kernel(const T* __restrict__ dy, const T* __restrict__ dr,
 // waits for its end on the device.
 template <typename W>
 __global__ void __launch_bounds__(256)
-add_rms_norm_dw_kernel(const float* __restrict__ partial, int parts, int H, W* __restrict__ dw) {
+add_rms_norm_dw_kernel(const float* partial, int parts, int H, W* __restrict__ dw) {
     __shared__ float sum[8][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    next_may_begin();
+    previous_done();
     float s = 0.f;
     if (c < H) {
 #pragma unroll 16
@@ -637,42 +645,29 @@ static int launch_norm(const void* x, const void* residual, const void* weight, 
     const int n = vec ? H / V : H;
     auto go = [&](auto kernel, int threads, int rows_per_cta, int ctas_per_sm) {
         const int need = (rows + rows_per_cta - 1) / rows_per_cta, most = sms * ctas_per_sm;
-        kernel<<<need < most ? need : most, threads, 0, st>>>(static_cast<const T*>(x), static_cast<const T*>(residual),
-                                                              static_cast<const W*>(weight), rows, H, eps,
-                                                              static_cast<T*>(r_out), out);
+        return launch_early(kernel, dim3(need < most ? need : most), threads, 0, 0, st, static_cast<const T*>(x),
+                            static_cast<const T*>(residual), static_cast<const W*>(weight), rows, H, eps,
+                            static_cast<T*>(r_out), out);
     };
     switch (plan) {
-        case NormPlan::VEC_FEW: go(add_rms_norm_kernel<T, W, V, 1, 1024, false, MX>, round_threads(n, 1), 1, 1); break;
-        case NormPlan::VEC_FEW2: go(add_rms_norm_kernel<T, W, V, 2, 1024, false, MX>, round_threads(n, 2), 1, 1); break;
+        case NormPlan::VEC_FEW: return go(add_rms_norm_kernel<T, W, V, 1, 1024, false, MX>, round_threads(n, 1), 1, 1);
+        case NormPlan::VEC_FEW2: return go(add_rms_norm_kernel<T, W, V, 2, 1024, false, MX>, round_threads(n, 2), 1, 1);
         case NormPlan::VEC_MANY: {
             const int threads = round_threads(n, 4);
-            go(add_rms_norm_kernel<T, W, V, 4, 256, false, MX>, threads, 1, 512 / threads);
-            break;
+            return go(add_rms_norm_kernel<T, W, V, 4, 256, false, MX>, threads, 1, 512 / threads);
         }
-        case NormPlan::VEC_MANY512: go(add_rms_norm_kernel<T, W, V, 4, 512, false, MX>, round_threads(n, 4), 1, 1); break;
-        case NormPlan::VEC_WARP: go(add_rms_norm_kernel<T, W, V, 4, 256, true, MX>, 256, 8, 2); break;
-        default:
-            if constexpr (!MX) {
-                if (plan == NormPlan::ONE_FEW) {
-                    go(add_rms_norm_kernel<T, W, 1, 8, 1024, false, false>, round_threads(n, 8), 1, 1);
-                    break;
-                }
-                if (plan == NormPlan::ONE_MANY) {
-                    go(add_rms_norm_kernel<T, W, 1, 16, 512, false, false>, round_threads(n, 16), 1,
-                       1024 / round_threads(n, 16));
-                    break;
-                }
-                if (plan == NormPlan::ONE_WARP) {
-                    go(add_rms_norm_kernel<T, W, 1, 8, 256, true, false>, 256, 8, 4);
-                    break;
-                }
-            }
-            add_rms_norm_wide_kernel<T, W, MX><<<rows < 8 * sms ? rows : 8 * sms, NORM_THREADS, 0, st>>>(
-                static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const W*>(weight), rows, H, eps,
-                static_cast<T*>(r_out), out);
+        case NormPlan::VEC_MANY512: return go(add_rms_norm_kernel<T, W, V, 4, 512, false, MX>, round_threads(n, 4), 1, 1);
+        case NormPlan::VEC_WARP: return go(add_rms_norm_kernel<T, W, V, 4, 256, true, MX>, 256, 8, 2);
+        default: break;
     }
-    DK_CUDA_OK(cudaGetLastError());
-    return DK_OK;
+    if constexpr (!MX) {
+        const int threads = round_threads(n, 16);
+        if (plan == NormPlan::ONE_FEW) return go(add_rms_norm_kernel<T, W, 1, 8, 1024, false, false>, round_threads(n, 8), 1, 1);
+        if (plan == NormPlan::ONE_MANY)
+            return go(add_rms_norm_kernel<T, W, 1, 16, 512, false, false>, threads, 1, 1024 / threads);
+        if (plan == NormPlan::ONE_WARP) return go(add_rms_norm_kernel<T, W, 1, 8, 256, true, false>, 256, 8, 4);
+    }
+    return go(add_rms_norm_wide_kernel<T, W, MX>, NORM_THREADS, 1, 8);
 }
 template <bool MX>
 static int launch_norm(const void* x, const void* residual, const void* weight, int x_is_f32, int w_is_f32, int T, int H,
@@ -700,46 +695,36 @@ static int launch_norm_bwd(const void* dy, const void* dr, const void* r, const 
         return parts = need < most ? need : most;
     };
     auto go = [&](auto kernel, int threads, int rows_per_cta, int ctas_per_sm) {
-        kernel<<<grid(rows_per_cta, ctas_per_sm), threads, shape.smem, st>>>(
-            static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r), rstd,
-            static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial, shape.ring);
+        return launch_early(kernel, dim3(grid(rows_per_cta, ctas_per_sm)), threads, shape.smem, 0, st,
+                            static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r), rstd,
+                            static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial, shape.ring);
     };
+    int done_rc = DK_OK;
     switch (plan) {
-        case NormPlan::VEC_FEW: go(add_rms_norm_bwd_kernel<T, W, V, 1, 1024, FROM_REGS>, round_threads(n, 1), 1, 1); break;
-        case NormPlan::VEC_FEW2: go(add_rms_norm_bwd_kernel<T, W, V, 2, 1024, FROM_REGS>, round_threads(n, 2), 1, 1); break;
+        case NormPlan::VEC_FEW: done_rc = go(add_rms_norm_bwd_kernel<T, W, V, 1, 1024, FROM_REGS>, round_threads(n, 1), 1, 1); break;
+        case NormPlan::VEC_FEW2: done_rc = go(add_rms_norm_bwd_kernel<T, W, V, 2, 1024, FROM_REGS>, round_threads(n, 2), 1, 1); break;
         case NormPlan::VEC_MANY: {
             const auto kernel = add_rms_norm_bwd_kernel<T, W, V, 4, 256, FROM_RING>;
-            static bool done[64] = {false};
-            int rc2 = allow_smem(kernel, done);
-            if (rc2 == DK_OK) rc2 = ring_shape(n, H, sizeof(T), dr != nullptr ? 3 : 2, &shape);
-            if (rc2 != DK_OK) return rc2;
-            go(kernel, shape.threads, 1, shape.ctas);
+            static bool allowed[64] = {false};
+            done_rc = allow_smem(kernel, allowed);
+            if (done_rc == DK_OK) done_rc = ring_shape(n, H, sizeof(T), dr != nullptr ? 3 : 2, &shape);
+            if (done_rc == DK_OK) done_rc = go(kernel, shape.threads, 1, shape.ctas);
             break;
         }
-        case NormPlan::VEC_MANY512: go(add_rms_norm_bwd_kernel<T, W, V, 4, 512, FROM_REGS>, round_threads(n, 4), 1, 1); break;
-        case NormPlan::VEC_WARP: go(add_rms_norm_bwd_kernel<T, W, V, 4, 256, FROM_WARP>, 256, 8, 2); break;
-        case NormPlan::ONE_FEW: go(add_rms_norm_bwd_kernel<T, W, 1, 8, 1024, FROM_REGS>, round_threads(n, 8), 1, 1); break;
-        case NormPlan::ONE_MANY: go(add_rms_norm_bwd_kernel<T, W, 1, 16, 512, FROM_REGS>, round_threads(n, 16), 1, 2); break;
-        case NormPlan::ONE_WARP: go(add_rms_norm_bwd_kernel<T, W, 1, 8, 256, FROM_WARP>, 256, 8, 2); break;
+        case NormPlan::VEC_MANY512: done_rc = go(add_rms_norm_bwd_kernel<T, W, V, 4, 512, FROM_REGS>, round_threads(n, 4), 1, 1); break;
+        case NormPlan::VEC_WARP: done_rc = go(add_rms_norm_bwd_kernel<T, W, V, 4, 256, FROM_WARP>, 256, 8, 2); break;
+        case NormPlan::ONE_FEW: done_rc = go(add_rms_norm_bwd_kernel<T, W, 1, 8, 1024, FROM_REGS>, round_threads(n, 8), 1, 1); break;
+        case NormPlan::ONE_MANY: done_rc = go(add_rms_norm_bwd_kernel<T, W, 1, 16, 512, FROM_REGS>, round_threads(n, 16), 1, 2); break;
+        case NormPlan::ONE_WARP: done_rc = go(add_rms_norm_bwd_kernel<T, W, 1, 8, 256, FROM_WARP>, 256, 8, 2); break;
         case NormPlan::WIDE:
-            add_rms_norm_bwd_wide_kernel<T, W><<<grid(1, 2), NORM_THREADS, 0, st>>>(
-                static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r), rstd,
-                static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial);
+            done_rc = launch_early(add_rms_norm_bwd_wide_kernel<T, W>, dim3(grid(1, 2)), NORM_THREADS, 0, 0, st,
+                                   static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r), rstd,
+                                   static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial);
             break;
     }
-    DK_CUDA_OK(cudaGetLastError());
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((H + 31) / 32);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    DK_CUDA_OK(cudaLaunchKernelEx(&cfg, add_rms_norm_dw_kernel<W>, static_cast<const float*>(partial), parts, H,
-                                  static_cast<W*>(dw)));
-    return DK_OK;
+    if (done_rc != DK_OK) return done_rc;
+    return launch_early(add_rms_norm_dw_kernel<W>, dim3((H + 31) / 32), 256, 0, 0, st, static_cast<const float*>(partial), parts, H,
+                        static_cast<W*>(dw));
 }
 
 }  // namespace dk

@@ -227,6 +227,63 @@ def test_two_streams_at_once_and_graph(T):
             assert all(torch.equal(u, v) for u, v in zip(out, w))
 
 
+@pytest.mark.parametrize("T", [3, 260])
+def test_order_with_other_work(T):
+    """The calls may set themselves up while earlier work runs, but read and write in order: after copies, memsets, torch's
+    kernels and events of another stream, before torch's kernels, over buffers that are used again and again, eager and
+    captured."""
+    import tk_kernel as tk
+    x, w13, w2, dy = (t.cuda() for t in make(T, 1024, 512, seed=5))
+    w = torch.ones(1024, dtype=torch.bfloat16, device="cuda")
+    want = []
+    for k in range(3):
+        a, _, rstd = tk.add_rms_norm(x * (k + 1), None, w)
+        torch.cuda.synchronize()
+        y, gu, h = tk.gated_ffn(a, w13, w2, True)
+        torch.cuda.synchronize()
+        g = tk.gated_ffn_bwd(dy, a, w13, w2, gu, h)
+        torch.cuda.synchronize()
+        d = tk.add_rms_norm_bwd(g[0], None, x * (k + 1), rstd, w)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in (y, *g, *d)])
+    side = torch.cuda.Stream()
+    buf, wbuf = torch.empty_like(x), torch.empty_like(w13)
+
+    def run(k):
+        buf.zero_()
+        wbuf.fill_(float("nan"))
+        buf.copy_(x)                                 # a copy, not a kernel
+        buf.mul_(k + 1)
+        ready = torch.cuda.Event()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            wbuf.copy_(w13)
+            ready.record(side)
+        a, _, rstd = tk.add_rms_norm(buf, None, w)
+        torch.cuda.current_stream().wait_event(ready)
+        y, gu, h = tk.gated_ffn(a, wbuf, w2, True)
+        g = tk.gated_ffn_bwd(dy, a, wbuf, w2, gu, h)
+        wbuf.mul_(2)                                 # written right behind its last reader
+        d = tk.add_rms_norm_bwd(g[0], None, buf, rstd, w)
+        out = [t * 1 for t in (y, *g, *d)]
+        buf.zero_()
+        return out
+
+    for _ in range(3):
+        got = [run(k) for k in range(3)]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [run(k) for k in range(3)]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
 def test_gradients_against_differences(orc):
     """The backward pass against central differences of the 64-bit forward along random directions."""
     import tk_kernel as tk
