@@ -473,13 +473,12 @@ __global__ void __launch_bounds__(THREADS, 1) ffn_gemm_kernel(const __grid_const
 //   EPI_GATED   a tile is 64 gate rows and the 64 up rows of the same columns; silu(g) * u leaves as h
 //   EPI_STORE   y from h and W2, or dx from [dg|du] and W13 (MN-major: 128 columns of W13)
 //   EPI_DGATED  dh from dy and W2 (MN-major: 128 columns of W2), with the kept g, u straight into dg, du
-// Half of the time of a small product is its beginning and its end, when HBM is idle; see the producer for what it does
-// meanwhile.
+// A product that follows another of the same call fills its ring with weights while that one ends. (More of them sent
+// to L2 ahead gained nothing: HBM is busy from the first CTA's start.)
 constexpr int ROWS_THREADS = 192;
 constexpr int ROWS_W_BYTES = 128 * BK * 2;
 // Shared memory of the ring: two CTAs on an SM up to 128 tokens, one above. The partial sums reuse it: N * 512 bytes.
 constexpr int ROWS_MAX_STAGES = 8;
-constexpr int64_t ROWS_PREFETCH = 32 << 20;  // bytes of weights that go to L2 ahead: what HBM delivers in 5 us
 __host__ __device__ constexpr int rows_ring(int N) { return N <= 128 ? 110 * 1024 : 208 * 1024; }
 constexpr int rows_smem(int N) { return 1024 + rows_ring(N) + 256; }
 static_assert(128 * 512 <= rows_ring(128) && 256 * 512 <= rows_ring(256), "the partial sums reuse the ring");
@@ -489,17 +488,11 @@ struct RowsMaps {
 struct RowsArgs {
     int N;                // tokens of a tile, a multiple of 16
     int weights_ready;    // the kernel before this one belongs to the same call
-    int prefetch;         // K blocks of weights that go to L2 ahead
     int T, cols, num_kb;  // cols: columns of the output (GATED, DGATED: F)
     __nv_bfloat16* out;   // [T, cols]; DGATED: [T, 2 cols]
     float* gu;            // [T, 2 cols]; GATED: written, may be null; DGATED: read
     unsigned* status;
 };
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* m, int x, int y) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x),
-                 "r"(y)
-                 : "memory");
-}
 __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
     float2 v;
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
@@ -557,7 +550,6 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
             cluster_wait();
         }
     };
-    next_may_begin();
 
     if (warp == 0) {  // whole warps, one elected thread: as in ffn_gemm_kernel
         auto load_w = [&](int kb, int s) {
@@ -579,25 +571,13 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
         };
         const int ahead = min(kb1 - kb0, stages);
         if (elect_one()) {
-            // While an earlier kernel still runs, its end being bound by a few CTAs, HBM is free. After a kernel of the same
-            // call, which writes no weights, the ring takes its first stages of them and L2 the next ones; otherwise L2 all.
-            const int first = g.weights_ready ? ahead : 0;
-            for (int i = 0; i < first; ++i) load_w(kb0 + i, i);
-            const int last = min(kb1, kb0 + first + g.prefetch);
-            for (int kb = kb0 + first; kb < last; ++kb) {
-                if (GATED) {
-                    tma_prefetch_2d(&maps.w, kb * BK, tile * 64);
-                    tma_prefetch_2d(&maps.w, kb * BK, g.cols + tile * 64);
-                } else if (W_MN) {
-                    tma_prefetch_2d(&maps.w, tile * 128, kb * BK);
-                    tma_prefetch_2d(&maps.w, tile * 128 + 64, kb * BK);
-                } else {
-                    tma_prefetch_2d(&maps.w, kb * BK, tile * 128);
-                }
-            }
+            // A kernel of the same call writes no weights, and it let this one begin only when all before it was complete:
+            // the ring takes its first stages of weights while that kernel ends.
+            for (int i = 0; i < ahead && g.weights_ready; ++i) load_w(kb0 + i, i);
         }
         __syncwarp();
         previous_done();
+        next_may_begin();  // not before: the next kernel may load weights at once
         asm volatile("fence.proxy.async;" ::: "memory");  // what earlier kernels wrote, for the copy engine
         if (elect_one()) {
             for (int i = 0; i < ahead; ++i) {
@@ -919,7 +899,6 @@ static int rows_product(const void* x, const void* W, void* out, int T, int cols
     int S = 1;
     while (S < 8 && tiles * token_tiles * S * 2 <= places && g.num_kb >= S * 4) S *= 2;
     g.weights_ready = follows;
-    g.prefetch = static_cast<int>(std::min<int64_t>(g.num_kb, ROWS_PREFETCH / (static_cast<int64_t>(tiles) * S * ROWS_W_BYTES)));
     return launch_early(kernel, dim3(tiles * S, token_tiles), ROWS_THREADS, rows_smem(N), S, st, maps, g);
 }
 

@@ -3,8 +3,9 @@
 //   - every thread that reads or writes global memory passes previous_done() first (or hangs, through a barrier in
 //     shared memory, on a thread that has), and every CTA passes it: when it returns, all kernels before this one on
 //     the stream are complete and what they wrote is visible;
-//   - before it a kernel only sets itself up, prefetches into L2 (where data cannot be stale), or loads what no
-//     kernel since the last full boundary writes;
+//   - before it a kernel only sets itself up. A kernel whose predecessor is known (one of the same call) may also load
+//     what that predecessor does not write, provided the predecessor says next_may_begin() after its own
+//     previous_done(): said earlier, kernels before the predecessor may still be running;
 //   - next_may_begin() says that the following kernel may set itself up too. A kernel that was not launched in this
 //     way starts after the end of this one, as ever.
 // After anything but a kernel (a copy, an event of another stream) the boundary is a full one.

@@ -284,6 +284,45 @@ def test_order_with_other_work(T):
             assert all(torch.equal(u, v) for u, v in zip(a, b))
 
 
+def test_weights_written_right_before(pkg):
+    """Weights that a kernel of this library writes right before the call: the second product's early loads of W2 (and of W13 in
+    the backward pass) come after that."""
+    import tk_kernel as tk
+    T, H, F = 5, 64, 8192
+    x, w13, w2, dy = (t.cuda() for t in make(T, H, F, seed=8))
+    ones, ones_h = (torch.ones(n, dtype=torch.bfloat16, device="cuda") for n in (F, H))
+    w2_rows = [(w2 * (k + 1) + k) for k in range(4)]
+    w13_rows = [(w13 * (k + 1) - k) for k in range(4)]
+    want = []
+    for a, b in zip(w2_rows, w13_rows):
+        n2, n13 = tk.add_rms_norm(a, None, ones)[0], tk.add_rms_norm(b, None, ones_h)[0]
+        torch.cuda.synchronize()
+        y, gu, h = tk.gated_ffn(x, n13, n2, True)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in (y, *tk.gated_ffn_bwd(dy, x, n13, n2, gu, h))])
+        torch.cuda.synchronize()
+    L, st = capi_lib(), torch.cuda.current_stream().cuda_stream
+    n2, n13, keep = torch.empty_like(w2), torch.empty_like(w13), torch.empty(F * 2, device="cuda")
+    for _ in range(20):
+        for k in range(4):
+            # into the same two buffers every time
+            assert L.dk_add_rms_norm(w13_rows[k].data_ptr(), None, ones_h.data_ptr(), 0, 0, 2 * F, H, 1e-6, n13.data_ptr(), None,
+                                     keep.data_ptr(), st) == 0
+            assert L.dk_add_rms_norm(w2_rows[k].data_ptr(), None, ones.data_ptr(), 0, 0, H, F, 1e-6, n2.data_ptr(), None,
+                                     keep.data_ptr(), st) == 0
+            y, gu, h = tk.gated_ffn(x, n13, n2, True)
+            assert L.dk_add_rms_norm(w13_rows[k].data_ptr(), None, ones_h.data_ptr(), 0, 0, 2 * F, H, 1e-6, n13.data_ptr(), None,
+                                     keep.data_ptr(), st) == 0
+            got = (y, *tk.gated_ffn_bwd(dy, x, n13, n2, gu, h))
+            for a, b in zip(got, want[k]):
+                assert torch.equal(a, b)
+
+
+def capi_lib():
+    from distributed_hipkittens_b200 import capi
+    return capi.lib()
+
+
 def test_gradients_against_differences(orc):
     """The backward pass against central differences of the 64-bit forward along random directions."""
     import tk_kernel as tk
