@@ -63,7 +63,8 @@ def bounds(x, w13, w2, dy):
 # one token to several tiles; rows and widths that end inside a tile; single vectors
 SHAPES = [(1, 512, 256), (2, 64, 64), (3, 8, 8), (5, 256, 72), (16, 1032, 136), (17, 520, 1000), (31, 2048, 4096), (33, 72, 2056),
           (64, 4096, 512), (65, 128, 128), (100, 512, 768), (127, 136, 264), (128, 256, 256), (129, 384, 640), (200, 1024, 136),
-          (255, 264, 392), (257, 320, 1288), (513, 512, 520), (700, 2056, 1032)]
+          (255, 264, 392), (257, 320, 1288), (513, 512, 520), (700, 2056, 1032),
+          (1000, 4104, 1544), (1357, 2048, 3592), (600, 3592, 5128), (2100, 2056, 2568)]
 
 
 @pytest.mark.parametrize("T,H,F", SHAPES)
@@ -152,13 +153,15 @@ def test_non_finite_rows_stay_in_their_rows(orc):
 
 
 def test_rows_do_not_depend_on_their_batch_neighbours(orc):
-    """Within one batch size a row's result depends on that row alone."""
+    """A row's result depends on that row and its place alone."""
     import tk_kernel as tk
-    for T in (7, 150, 400):
-        x, w13, w2, _ = make(T, 512, 264)
-        a = tk.gated_ffn(x.cuda(), w13.cuda(), w2.cuda())
-        b = tk.gated_ffn(x.flip(0).contiguous().cuda(), w13.cuda(), w2.cuda())
-        assert torch.equal(a, b.flip(0))
+    for T, H, F in ((7, 512, 264), (150, 512, 264), (400, 512, 264), (1357, 2048, 1032)):
+        x, w13, w2, _ = make(T, H, F)
+        other = make(T, H, F, seed=1)[0]
+        keep = torch.arange(0, T, 3)
+        other[keep] = x[keep]
+        a, b = (tk.gated_ffn(t.cuda(), w13.cuda(), w2.cuda()) for t in (x, other))
+        assert torch.equal(a[keep], b[keep]) and not torch.equal(a, b)
 
 
 def test_no_rows():
@@ -171,9 +174,8 @@ def test_no_rows():
     assert dx.shape == (0, 64) and (dw13 == 0).all() and (dw2 == 0).all() and dw13.shape == w13.shape and dw2.shape == w2.shape
 
 
-@pytest.mark.parametrize("T", [1, 37, 300])
-def test_nothing_is_written_outside(capi, T):
-    H, F = 136, 200
+@pytest.mark.parametrize("T,H,F", [(1, 136, 200), (37, 136, 200), (300, 136, 200), (1357, 2056, 1032)])
+def test_nothing_is_written_outside(capi, T, H, F):
     x, w13, w2, dy = (t.cuda() for t in make(T, H, F))
     L, st = capi.lib(), capi._stream_ptr(None)
     sizes = dict(gu=8 * T * F, h=2 * T * F, y=2 * T * H, dgu=4 * T * F, dx=2 * T * H, dw13=4 * F * H, dw2=2 * F * H)
