@@ -637,6 +637,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
             }
         }
     } else if (warp == 1) {
+        previous_done();  // before any bounded wait: its limit is not for the kernel before
         const uint32_t idesc = umma_idesc(1, 1, 128, N) | (W_MN ? 1u << 15 : 0u);
         constexpr uint64_t w_step = W_MN ? 16 * 128 / 16 : 2;
         int s = 0;
@@ -664,6 +665,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
         if (ok && elect_one()) umma_commit<1>(bar_done);
     } else {
         // partial sums as [token][weight row]; every load has been consumed, so the ring is free
+        previous_done();
         const int q = warp & 3;
         if (__all_sync(0xffffffffu, mbar_wait(bar_done, 0, wc, SITE_TMEM_FULL, tile))) {
             tc_fence_after();
@@ -682,7 +684,6 @@ __global__ void __launch_bounds__(ROWS_THREADS) ffn_rows_kernel(const __grid_con
         }
     }
     tc_fence_before();
-    previous_done();  // for every thread that writes, or reads the kept g and u
     meet();
     {
         constexpr int PAIRS = GATED ? 32 : 64;  // pairs of neighbouring output columns of a tile

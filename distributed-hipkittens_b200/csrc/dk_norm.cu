@@ -580,6 +580,16 @@ static int check_norm(const void* x, const void* weight, int x_is_f32, int w_is_
     DK_REQUIRE(w_is_f32 || !x_is_f32, "a bf16 weight needs bf16 rows");
     return DK_OK;
 }
+// Every element on its own size: what any path needs. (16 bytes only choose the faster one.)
+static int check_elements(int x_is_f32, int w_is_f32, std::initializer_list<const void*> rows, const void* weight,
+                          std::initializer_list<const void*> f32) {
+    uintptr_t row_bits = 0, f32_bits = 0;
+    for (const void* p : rows) row_bits |= reinterpret_cast<uintptr_t>(p);
+    for (const void* p : f32) f32_bits |= reinterpret_cast<uintptr_t>(p);
+    DK_REQUIRE((row_bits & (x_is_f32 ? 3 : 1)) == 0 && (reinterpret_cast<uintptr_t>(weight) & (w_is_f32 ? 3 : 1)) == 0 &&
+                   (f32_bits & 3) == 0, "a tensor does not start on a whole element");
+    return DK_OK;
+}
 
 // How a pass over T rows of H elements is cut up.
 //   vec      16-byte accesses: every row and the weight start on 16 bytes
@@ -738,6 +748,8 @@ extern "C" int dk_add_rms_norm(const void* x, const void* residual, const void* 
     if (T == 0) return DK_OK;
     DK_REQUIRE(y != nullptr, "null output");
     DK_REQUIRE((residual != nullptr) == (r_out != nullptr), "r_out goes with a residual, and a residual with r_out");
+    const int rc2 = check_elements(x_is_f32, w_is_f32, {x, residual, y, r_out}, weight, {rstd});
+    if (rc2 != DK_OK) return rc2;
     return launch_norm<false>(x, residual, weight, x_is_f32, w_is_f32, T, H, eps, r_out,
                               NormOut{y, rstd, nullptr, nullptr, nullptr}, static_cast<cudaStream_t>(stream));
 }
@@ -754,6 +766,8 @@ extern "C" int dk_add_rms_norm_mx(const void* x, const void* residual, const voi
     DK_REQUIRE((residual != nullptr) == (r_out != nullptr), "r_out goes with a residual, and a residual with r_out");
     DK_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(s_rows) | reinterpret_cast<uintptr_t>(sf_atoms)) & 15) == 0,
                "q, s_rows and sf_atoms must be 16-byte aligned");
+    const int rc2 = check_elements(x_is_f32, w_is_f32, {x, residual, r_out}, weight, {});
+    if (rc2 != DK_OK) return rc2;
     return launch_norm<true>(x, residual, weight, x_is_f32, w_is_f32, T, H, eps, r_out,
                              NormOut{nullptr, nullptr, static_cast<uint8_t*>(q), static_cast<uint8_t*>(s_rows),
                                      static_cast<uint8_t*>(sf_atoms)},
@@ -782,6 +796,9 @@ extern "C" int dk_add_rms_norm_bwd(const void* dy, const void* dr, const void* r
     DK_REQUIRE(dx != nullptr, "null output");
     DK_REQUIRE(workspace != nullptr && workspace_bytes >= dk_add_rms_norm_bwd_workspace_bytes(T, H), "workspace too small");
     DK_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "the workspace must be 16-byte aligned");
+    const int rc2 = check_elements(x_is_f32, w_is_f32, {dy, dr, r, dx}, weight, {rstd});
+    if (rc2 != DK_OK) return rc2;
+    DK_REQUIRE((reinterpret_cast<uintptr_t>(dw) & (w_is_f32 ? 3 : 1)) == 0, "a tensor does not start on a whole element");
     float* partial = static_cast<float*>(workspace);
     if (x_is_f32) return launch_norm_bwd<float, float>(dy, dr, r, rstd, weight, T, H, dx, dw, partial, st);
     if (w_is_f32) return launch_norm_bwd<__nv_bfloat16, float>(dy, dr, r, rstd, weight, T, H, dx, dw, partial, st);

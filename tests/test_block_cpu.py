@@ -46,7 +46,7 @@ def test_c_abi_argument_errors(capi):
     norm = lambda T=4, H=64, x=one, w=one, xf=0, wf=0, eps=1e-6, y=one, res=None, r=None: L.dk_add_rms_norm(
         x, res, w, xf, wf, T, H, eps, y, r, one, None)
     bad = [norm(T=-1), norm(H=0), norm(H=65537), norm(x=None), norm(w=None), norm(y=None), norm(xf=1, wf=0), norm(eps=0.0),
-           norm(eps=-1.0), norm(eps=float("nan")), norm(eps=float("inf")), norm(res=one), norm(r=one)]
+           norm(eps=-1.0), norm(eps=float("nan")), norm(eps=float("inf")), norm(res=one), norm(r=one), norm(x=_p(4097)), norm(y=_p(4097)), norm(w=_p(4097)), norm(x=_p(4098), xf=1, wf=1)]
     assert bad == [capi.ERR_ARG] * len(bad)
     assert norm(T=0, x=None, y=None) == 0
     mx = lambda T=4, H=128, q=one, s=one, a=one, res=None, r=None: L.dk_add_rms_norm_mx(one, res, one, 0, 0, T, H, 1e-6, q, s, a,
@@ -59,7 +59,7 @@ def test_c_abi_argument_errors(capi):
     bwd = lambda dy=one, r=one, rstd=one, w=one, dx=one, dw=one, ws=one, n=wb: L.dk_add_rms_norm_bwd(
         dy, None, r, rstd, w, 0, 0, 4, 64, dx, dw, ws, n, None)
     bad = [bwd(dy=None), bwd(r=None), bwd(rstd=None), bwd(w=None), bwd(dx=None), bwd(dw=None), bwd(ws=None), bwd(n=wb - 1),
-           bwd(ws=_p(4100))]
+           bwd(ws=_p(4100)), bwd(dy=_p(4097)), bwd(dx=_p(4097)), bwd(rstd=_p(4098)), bwd(dw=_p(4097))]
     assert bad == [capi.ERR_ARG] * len(bad)
     ffn = lambda T=4, H=64, F=32, x=one, w13=one, w2=one, h=one, y=one: L.dk_gated_ffn(x, w13, w2, T, H, F, None, h, y, None)
     bad = [ffn(T=-1), ffn(H=0), ffn(F=0), ffn(H=60), ffn(F=20), ffn(x=None), ffn(w13=None), ffn(w2=None), ffn(h=None), ffn(y=None),

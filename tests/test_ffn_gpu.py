@@ -25,6 +25,12 @@ pytestmark = pytest.mark.gpu
 R = 2.0 ** -8 / 3 ** 0.5
 
 
+@pytest.fixture(scope="module")
+def ops(pkg):
+    from distributed_hipkittens_b200 import torch_ops
+    return torch.ops.dk_b200
+
+
 def make(T, H, F, seed=0):
     g = torch.Generator().manual_seed(seed + T + 7 * H + 31 * F)
     n = lambda *s, std=1.0: (torch.randn(*s, generator=g) * std).to(torch.bfloat16)
@@ -189,6 +195,51 @@ def test_nothing_is_written_outside(capi, T, H, F):
         assert (b[:4096] == 0xA5).all() and (b[4096 + sizes[k]:] == 0xA5).all(), k
 
 
+def test_more_than_2_31_elements(capi):
+    """Offsets past 32 bits: [g|u] and its gradient have 2.3e9 elements. The last rows of y and dx against the formulas, and some
+    columns of the weight gradients, sums over all rows."""
+    import tk_kernel as tk
+    T, H, F = 70000, 64, 16384
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n = lambda *s, std=1.0: (torch.randn(*s, generator=g, device="cuda") * std).to(torch.bfloat16)
+    x, w13, w2, dy = n(T, H), n(2 * F, H, std=H ** -0.5), n(H, F, std=F ** -0.5), n(T, H)
+    y, gu, h = tk.gated_ffn(x, w13, w2, True)
+    dx, dw13, dw2 = tk.gated_ffn_bwd(dy, x, w13, w2, gu, h)
+    torch.cuda.synchronize()
+    assert capi.device_status()[0] == 0
+    assert 2 * T * F > 1 << 31
+    last = slice(T - 40, T)
+    a = x[last].double()
+    gate, up = (a @ w13.double().t()).chunk(2, 1)
+    s = torch.sigmoid(gate)
+    h64 = gate * s * up
+    near(h[last], h64, 1)
+    near(y[last], h64 @ w2.double().t(), 2)
+    dh = dy[last].double() @ w2.double()
+    dgu = torch.cat([dh * up * (s + gate * s * (1 - s)), dh * gate * s], 1)
+    near(dx[last], dgu @ w13.double(), 2)
+    cols = torch.tensor([0, 1, F // 2, F - 1], device="cuda")
+    gate, up = (x.double() @ w13[c].double().t() for c in (cols, F + cols))
+    s = torch.sigmoid(gate)
+    dh = dy.double() @ w2[:, cols].double()
+    near(dw2[:, cols], dy.double().t() @ (gate * s * up), 2)
+    near(dw13[cols], (dh * up * (s + gate * s * (1 - s))).t() @ x.double(), 2)
+    near(dw13[F + cols], (dh * gate * s).t() @ x.double(), 2)
+    del y, gu, h, dx
+    torch.cuda.empty_cache()
+
+
+def test_operators_pass_opcheck(ops):
+    x, w13, w2, dy = (t.cuda() for t in make(20, 128, 72))
+    w = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    y, r, rstd = ops.add_rms_norm(x, dy, w)
+    _, gu, h = ops.gated_ffn_train(x, w13, w2)
+    for op, args in ((ops.rms_norm, (x, w)), (ops.add_rms_norm, (x, dy, w)), (ops.add_rms_norm_bwd, (dy, None, r, rstd, w)),
+                     (ops.add_rms_norm_mx, (x, dy, w)), (ops.gated_ffn, (x, w13, w2)), (ops.gated_ffn_train, (x, w13, w2)),
+                     (ops.gated_ffn_bwd, (dy, x, w13, w2, gu, h))):
+        torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
+
+
 @pytest.mark.parametrize("T", [4, 260])
 def test_two_streams_at_once_and_graph(T):
     """Two calls that overlap on the GPU, and a captured step replayed on other inputs."""
@@ -343,12 +394,6 @@ def test_gradients_against_differences(orc):
         assert (got - slope).abs() <= 6 * 2 ** 0.5 * R * grad.double().norm() * args[i].std()
 
 
-@pytest.fixture(scope="module")
-def ops(pkg):
-    from distributed_hipkittens_b200 import torch_ops
-    return torch.ops.dk_b200
-
-
 def test_the_block_as_it_is_trained(ops, orc):
     """norm with residual -> feed-forward -> added to the stream by the next norm, gradients through autograd, against
     the same in 64 bits. Roundings on the way: the stream twice, the normed rows twice, h and y; the gradients pass
@@ -390,8 +435,6 @@ def test_autograd_alone(ops, orc):
     a, r, _ = ops.add_rms_norm(xr, x, w)
     gx, = torch.autograd.grad(r.sum(), [xr])           # only the stream is used
     assert (gx == 1).all()
-    torch.library.opcheck(ops.rms_norm.default, (x, w.detach()), test_utils=("test_schema", "test_faketensor"))
-    torch.library.opcheck(ops.gated_ffn_train.default, (x, w13, w2), test_utils=("test_schema", "test_faketensor"))
 
 
 def test_serving_run(capi, orc):
