@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 namespace dk {
 
@@ -34,38 +35,79 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// V consecutive elements as they lie in memory: one 2- or 4-byte access, or 16-byte ones.
+// V consecutive elements as they lie in memory, a multiple of 16 bytes.
 template <typename T, int V>
 struct Pack {
-    static constexpr int N16 = V * static_cast<int>(sizeof(T)) / 16;  // 16-byte accesses; 0: a single element
-    static_assert(V == 1 || V * sizeof(T) % 16 == 0, "whole 16-byte vectors, or one element");
+    static constexpr int N16 = V * static_cast<int>(sizeof(T)) / 16;
+    static_assert(N16 > 0 && V * sizeof(T) % 16 == 0, "whole 16-byte vectors");
     union {
-        uint4 v[N16 > 0 ? N16 : 1];
+        uint4 v[N16];
         T e[V];
     };
     __device__ __forceinline__ Pack() {}
     __device__ __forceinline__ void load(const T* p) {
-        if constexpr (N16 > 0) {
 #pragma unroll
-            for (int i = 0; i < N16; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
-        } else {
-            e[0] = *p;
-        }
+        for (int i = 0; i < N16; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
     }
     __device__ __forceinline__ void store(T* p) const {
-        if constexpr (N16 > 0) {
 #pragma unroll
-            for (int i = 0; i < N16; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
-        } else {
-            *p = e[0];
-        }
+        for (int i = 0; i < N16; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
     }
     __device__ __forceinline__ void zero() {
-        if constexpr (N16 > 0) {
 #pragma unroll
-            for (int i = 0; i < N16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < N16; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+};
+
+// The vectors of a row and the threads that have them: vector i begins at element i * V - shift of the row. Where every row
+// starts on 16 bytes (RAGGED == false) shift is 0 and vectors are whole. Otherwise rows start `shift` elements behind a
+// 16-byte boundary, their first and last vectors are partial (done element by element), all others are whole all the same.
+// Element r * H lies (r * H) % V behind a boundary; a CTA's rows are a multiple of V apart, so shift is the same for all of
+// them and what a thread keeps (the weight, its columns of dw) stays in place.
+template <int V, bool RAGGED>
+struct RowVectors {
+    int H, shift, count;
+    __device__ __forceinline__ RowVectors(int first_row, int H_) : H(H_) {
+        shift = RAGGED ? static_cast<int>(static_cast<int64_t>(first_row) * H_ % V) : 0;
+        count = RAGGED ? (H + shift + V - 1) / V : H / V;
+    }
+    __device__ __forceinline__ bool whole(int i) const { return !RAGGED || (i * V >= shift && (i + 1) * V - shift <= H); }
+    __device__ __forceinline__ bool has(int i, int k) const {
+        const int c = i * V + k - shift;
+        return !RAGGED || (c >= 0 && c < H);
+    }
+    // `row`: the row's first element
+    template <typename T>
+    __device__ __forceinline__ void load(Pack<T, V>& p, const T* row, int i) const {
+        const T* at = row + (static_cast<int64_t>(i) * V - shift);
+        if (whole(i)) {
+            p.load(at);
         } else {
-            e[0] = from_f32<T>(0.f);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (has(i, k)) p.e[k] = at[k];
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(const Pack<T, V>& p, T* row, int i) const {
+        T* at = row + (static_cast<int64_t>(i) * V - shift);
+        if (whole(i)) {
+            p.store(at);
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (has(i, k)) at[k] = p.e[k];
+        }
+    }
+    // the weight lies on a boundary whatever the row does
+    template <typename W>
+    __device__ __forceinline__ void load_weight(Pack<W, V>& p, const W* weight, int i) const {
+        if constexpr (!RAGGED) {
+            p.load(weight + static_cast<int64_t>(i) * V);
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (has(i, k)) p.e[k] = weight[i * V + k - shift];
         }
     }
 };
@@ -75,7 +117,7 @@ struct Pack {
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> added(const Pack<T, V>& a, const Pack<T, V>& b) {
     Pack<T, V> r;
-    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i)
             reinterpret_cast<__nv_bfloat162*>(r.e)[i] =
@@ -103,7 +145,7 @@ __device__ __forceinline__ float row_sum(float v, float (&part)[2][32], int whic
 }
 
 // How the values of a row reach the threads of a backward pass.
-//   FROM_REGS   each thread loads its own 16-byte vectors (or elements), those of the next row as soon as it has added
+//   FROM_REGS   each thread loads its own 16-byte vectors, those of the next row as soon as it has added
 //               up this row's: they are in flight during the reduction and the writing
 //   FROM_WARP   the same, a row to a warp: no barrier
 //   FROM_RING   one thread has whole rows copied into a ring in shared memory (cp.async.bulk), as many rows ahead as
@@ -213,10 +255,11 @@ struct NormOut {
 // narrow). CTAs are persistent: the weight is read once, and the next row's loads are issued as soon as this row's values
 // have been added up, so that they are in flight during the reduction and the writing of y. Every element is read once
 // and written once. NT: most threads that share a row.
-template <typename T, typename W, int V, int VPT, int NT, bool WARP, bool MX>
+template <typename T, typename W, int VPT, int NT, bool WARP, bool RAGGED, bool MX>
 __global__ void __launch_bounds__(NT)
 add_rms_norm_kernel(const T* x, const T* residual, const W* weight, int rows, int H, float eps, T* r_out,
                     const NormOut out) {
+    constexpr int V = 16 / sizeof(T);
     __shared__ float part[2][32];
     next_may_begin();
     previous_done();
@@ -224,7 +267,7 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* weight, int rows, in
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     const int stride = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
-    const int nvec = H / V;
+    const RowVectors<V, RAGGED> at(first, H);
     Pack<W, V> w[VPT];
     Pack<T, V> a[VPT], b[VPT];
     auto fetch = [&](int row) {
@@ -233,9 +276,9 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* weight, int rows, in
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int i = j * per_row + tid;
-            if (i < nvec) {
-                a[j].load(xr + static_cast<size_t>(i) * V);
-                if (residual != nullptr) b[j].load(rr + static_cast<size_t>(i) * V);
+            if (i < at.count) {
+                at.load(a[j], xr, i);
+                if (residual != nullptr) at.load(b[j], rr, i);
             }
         }
     };
@@ -248,7 +291,7 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* weight, int rows, in
     if (first < rows) fetch(first);
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
-        if (j * per_row + tid < nvec) w[j].load(weight + static_cast<size_t>(j * per_row + tid) * V);
+        if (j * per_row + tid < at.count) at.load_weight(w[j], weight, j * per_row + tid);
     if constexpr (MX) mx_clear_padding(out.atoms, rows, H, WARP ? blockDim.x : per_row);
     int which = 0;
     for (int row = first; row < rows; row += stride, which ^= 1) {
@@ -268,7 +311,7 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* weight, int rows, in
         if (residual != nullptr) {
 #pragma unroll
             for (int j = 0; j < VPT; ++j)
-                if (j * per_row + tid < nvec) r[j].store(r_out + base + static_cast<size_t>(j * per_row + tid) * V);
+                if (j * per_row + tid < at.count) at.store(r[j], r_out + base, j * per_row + tid);
         }
         const float rstd = rstd_of(row_sum<WARP>(ss, part, which, per_row), H, eps);
         if (out.rstd != nullptr && tid == 0) out.rstd[row] = rstd;
@@ -276,11 +319,11 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* weight, int rows, in
         for (int j = 0; j < VPT; ++j) {
             const int i = j * per_row + tid;
             if constexpr (!MX) {
-                if (i < nvec) {
+                if (i < at.count) {
                     Pack<T, V> y;
 #pragma unroll
                     for (int k = 0; k < V; ++k) y.e[k] = from_f32<T>(to_f32(r[j].e[k]) * rstd * to_f32(w[j].e[k]));
-                    y.store(static_cast<T*>(out.y) + base + static_cast<size_t>(i) * V);
+                    at.store(y, static_cast<T*>(out.y) + base, i);
                 }
             } else {
                 // 32 / V lanes hold a block of 32 values, 128 / V lanes the four blocks whose scale bytes are one
@@ -307,7 +350,7 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* weight, int rows, in
                 word |= __shfl_down_sync(0xffffffffu, word, BLOCK) << 8;
                 word |= __shfl_down_sync(0xffffffffu, word, 2 * BLOCK) << 16;
                 const int lane = threadIdx.x & 31, lead = lane & ~(WORD - 1);
-                if (i < nvec) {
+                if (i < at.count) {
                     uint32_t p[V / 4];
 #pragma unroll
                     for (int k = 0; k < V / 4; ++k) {
@@ -382,12 +425,14 @@ add_rms_norm_wide_kernel(const T* x, const T* residual, const W* weight, int row
 // Backward pass on the same plan, with the thread's columns of dw summed in registers over the CTA's rows. Each CTA
 // leaves one row of `partial` [gridDim.x][H]; every element is summed by one thread in row order: the same bits on
 // every run.
-template <typename T, typename W, int V, int VPT, int NT, int FROM>
+template <typename T, typename W, int VPT, int NT, int FROM, bool RAGGED>
 __global__ void __launch_bounds__(NT)
 add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
                         const float* rstd_in, const W* weight, int rows, int H,
                         T* dx, float* partial, const Ring ring) {
+    constexpr int V = 16 / sizeof(T);
     constexpr bool WARP = FROM == FROM_WARP, RING = FROM == FROM_RING;
+    static_assert(!(RING && RAGGED), "the ring copies rows that start on 16 bytes");
     __shared__ float part[2][32];
     __shared__ float warp_dw[WARP ? NT / 32 : 1][WARP ? 32 * VPT * V : 1];
     __shared__ RingShared sh;
@@ -396,7 +441,7 @@ add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
     const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int first = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
     const int stride = WARP ? gridDim.x * (blockDim.x >> 5) : gridDim.x;
-    const int nvec = H / V;
+    const RowVectors<V, RAGGED> at(first, H);
     next_may_begin();
     previous_done();
     const T* const src[3] = {dy, r, dr};
@@ -410,16 +455,16 @@ add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int i = j * per_row + tid;
-            if (i < nvec) {
-                a[j].load(p + static_cast<size_t>(i) * V);
-                b[j].load(q + static_cast<size_t>(i) * V);
+            if (i < at.count) {
+                at.load(a[j], p, i);
+                at.load(b[j], q, i);
             }
         }
     };
     auto fetch_above = [&](const T* p) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
-            if (j * per_row + tid < nvec) c[j].load(p + static_cast<size_t>(j * per_row + tid) * V);
+            if (j * per_row + tid < at.count) at.load(c[j], p, j * per_row + tid);
     };
     auto fetch_row = [&](int row) {
         fetch(dy + static_cast<size_t>(row) * H, r + static_cast<size_t>(row) * H);
@@ -438,7 +483,7 @@ add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
     if (!RING && first < rows) fetch_row(first);
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
-        if (j * per_row + tid < nvec) w[j].load(weight + static_cast<size_t>(j * per_row + tid) * V);
+        if (j * per_row + tid < at.count) at.load_weight(w[j], weight, j * per_row + tid);
     int which = 0;
     for (int row = first; row < rows; row += stride, which ^= 1) {
         const size_t base = static_cast<size_t>(row) * H;
@@ -470,7 +515,7 @@ add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int i = j * per_row + tid;
-            if (i < nvec) {
+            if (i < at.count) {
                 Pack<T, V> o;
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
@@ -479,7 +524,7 @@ add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
                     if (dr != nullptr) v += to_f32(c[j].e[k]);
                     o.e[k] = from_f32<T>(v);
                 }
-                o.store(dx + base + static_cast<size_t>(i) * V);
+                at.store(o, dx + base, i);
             }
         }
     }
@@ -489,7 +534,11 @@ add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
 #pragma unroll
-            for (int k = 0; k < V; ++k) warp_dw[threadIdx.x >> 5][(j * 32 + tid) * V + k] = dw[j][k];
+            for (int k = 0; k < V; ++k) {
+                // element (j * 32 + tid) * V + k - shift; a warp's shift is its own
+                const int col = (j * 32 + tid) * V + k - at.shift;
+                if (col >= 0 && col < H) warp_dw[threadIdx.x >> 5][col] = first < rows ? dw[j][k] : 0.f;
+            }
         __syncthreads();
         for (int col = threadIdx.x; col < H; col += blockDim.x) {
             float s = 0.f;
@@ -499,9 +548,10 @@ add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
     } else {
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
-            if (j * per_row + tid < nvec) {
+            if (j * per_row + tid < at.count) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) mine[static_cast<size_t>(j * per_row + tid) * V + k] = dw[j][k];
+                for (int k = 0; k < V; ++k)
+                    if (at.has(j * per_row + tid, k)) mine[(j * per_row + tid) * V + k - at.shift] = dw[j][k];
             }
     }
 }
@@ -591,26 +641,17 @@ static int check_elements(int x_is_f32, int w_is_f32, std::initializer_list<cons
     return DK_OK;
 }
 
-// How a pass over T rows of H elements is cut up.
-//   vec      16-byte accesses: every row and the weight start on 16 bytes
-//   few      at most one row for each SM: as many threads to a row as it can use (latency); otherwise four
-//            vectors a thread, so that a CTA has enough bytes in flight (bandwidth)
-//   warp     rows of at most 4 vectors (or 8 elements) a lane: a row to a warp, no barrier
-//   wide     a row that does not fit into the registers of 512 threads
-enum class NormPlan { VEC_FEW, VEC_FEW2, VEC_MANY, VEC_MANY512, VEC_WARP, ONE_FEW, ONE_MANY, ONE_WARP, WIDE };
-static NormPlan norm_plan(bool vec, int V, int T, int H, int sms) {
-    const int n = vec ? H / V : H;
-    const bool few = T <= sms;
-    if (vec) {
-        if (!few && n <= 128) return NormPlan::VEC_WARP;
-        if (few && n <= 1024) return NormPlan::VEC_FEW;
-        if (few && n <= 2048) return NormPlan::VEC_FEW2;
-        if (n <= 1024) return NormPlan::VEC_MANY;
-        return n <= 2048 ? NormPlan::VEC_MANY512 : NormPlan::WIDE;
-    }
-    if (!few && n <= 256) return NormPlan::ONE_WARP;
-    if (n > 8192) return NormPlan::WIDE;
-    return few ? NormPlan::ONE_FEW : NormPlan::ONE_MANY;
+// How a pass over T rows of H elements is cut up. n: vectors a row may span.
+//   FEW      at most one row for each SM: as many threads to a row as it can use (latency)
+//   MANY     four vectors a thread, so that a CTA has enough bytes in flight (bandwidth)
+//   WARP     rows of at most 4 vectors a lane: a row to a warp, no barrier
+//   WIDE     a row that does not fit into the registers of 512 threads, or tensors that do not start on 16 bytes
+enum class NormPlan { FEW, FEW2, MANY, MANY512, WARP, WIDE };
+static NormPlan norm_plan(bool aligned, int n, int T, int sms) {
+    if (!aligned || n > 2048) return NormPlan::WIDE;
+    if (T <= sms) return n <= 1024 ? NormPlan::FEW : NormPlan::FEW2;
+    if (n <= 128) return NormPlan::WARP;
+    return n <= 1024 ? NormPlan::MANY : NormPlan::MANY512;
 }
 // Launch shape of a ring kernel: threads that share a row, CTAs on an SM and the ring of each.
 struct RingShape {
@@ -650,32 +691,29 @@ static int launch_norm(const void* x, const void* residual, const void* weight, 
     int sms = 0;
     const int rc = sm_count(&sms);
     if (rc != DK_OK) return rc;
-    const bool vec = H % V == 0 && aligned16({x, residual, weight, r_out, out.y});
-    const NormPlan plan = norm_plan(vec, V, rows, H, sms);
-    const int n = vec ? H / V : H;
+    const bool ragged = H % V != 0;
+    const int n = ragged ? (H + 2 * V - 2) / V : H / V;
+    const NormPlan plan = norm_plan(aligned16({x, residual, weight, r_out, out.y}), n, rows, sms);
     auto go = [&](auto kernel, int threads, int rows_per_cta, int ctas_per_sm) {
-        const int need = (rows + rows_per_cta - 1) / rows_per_cta, most = sms * ctas_per_sm;
+        const int need = (rows + rows_per_cta - 1) / rows_per_cta, most = ragged ? sms * ctas_per_sm / V * V : sms * ctas_per_sm;
         return launch_early(kernel, dim3(need < most ? need : most), threads, 0, 0, st, static_cast<const T*>(x),
                             static_cast<const T*>(residual), static_cast<const W*>(weight), rows, H, eps,
                             static_cast<T*>(r_out), out);
     };
-    switch (plan) {
-        case NormPlan::VEC_FEW: return go(add_rms_norm_kernel<T, W, V, 1, 1024, false, MX>, round_threads(n, 1), 1, 1);
-        case NormPlan::VEC_FEW2: return go(add_rms_norm_kernel<T, W, V, 2, 1024, false, MX>, round_threads(n, 2), 1, 1);
-        case NormPlan::VEC_MANY: {
-            const int threads = round_threads(n, 4);
-            return go(add_rms_norm_kernel<T, W, V, 4, 256, false, MX>, threads, 1, 512 / threads);
+    auto planned = [&](auto is_ragged) {
+        constexpr bool R = decltype(is_ragged)::value;
+        switch (plan) {
+            case NormPlan::FEW: return go(add_rms_norm_kernel<T, W, 1, 1024, false, R, MX>, round_threads(n, 1), 1, 1);
+            case NormPlan::FEW2: return go(add_rms_norm_kernel<T, W, 2, 1024, false, R, MX>, round_threads(n, 2), 1, 1);
+            case NormPlan::MANY:
+                return go(add_rms_norm_kernel<T, W, 4, 256, false, R, MX>, round_threads(n, 4), 1, 512 / round_threads(n, 4));
+            case NormPlan::MANY512: return go(add_rms_norm_kernel<T, W, 4, 512, false, R, MX>, round_threads(n, 4), 1, 1);
+            default: return go(add_rms_norm_kernel<T, W, 4, 256, true, R, MX>, 256, 8, 2);
         }
-        case NormPlan::VEC_MANY512: return go(add_rms_norm_kernel<T, W, V, 4, 512, false, MX>, round_threads(n, 4), 1, 1);
-        case NormPlan::VEC_WARP: return go(add_rms_norm_kernel<T, W, V, 4, 256, true, MX>, 256, 8, 2);
-        default: break;
-    }
-    if constexpr (!MX) {
-        const int threads = round_threads(n, 16);
-        if (plan == NormPlan::ONE_FEW) return go(add_rms_norm_kernel<T, W, 1, 8, 1024, false, false>, round_threads(n, 8), 1, 1);
-        if (plan == NormPlan::ONE_MANY)
-            return go(add_rms_norm_kernel<T, W, 1, 16, 512, false, false>, threads, 1, 1024 / threads);
-        if (plan == NormPlan::ONE_WARP) return go(add_rms_norm_kernel<T, W, 1, 8, 256, true, false>, 256, 8, 4);
+    };
+    if (plan != NormPlan::WIDE) {
+        if (!ragged) return planned(std::false_type{});
+        if constexpr (!MX) return planned(std::true_type{});
     }
     return go(add_rms_norm_wide_kernel<T, W, MX>, NORM_THREADS, 1, 8);
 }
@@ -695,13 +733,14 @@ static int launch_norm_bwd(const void* dy, const void* dr, const void* r, const 
     const int rc = sm_count(&sms);
     if (rc != DK_OK) return rc;
     if (sms > NORM_MAX_SMS) sms = NORM_MAX_SMS;
-    const bool vec = H % V == 0 && aligned16({dy, dr, r, weight, dx});
-    const NormPlan plan = norm_plan(vec, V, rows, H, sms);
-    const int n = vec ? H / V : H;
+    const bool ragged = H % V != 0;
+    const int n = ragged ? (H + 2 * V - 2) / V : H / V;
+    const NormPlan plan = norm_plan(aligned16({dy, dr, r, weight, dx}), n, rows, sms);
     int parts = 0;
     RingShape shape{};
     auto grid = [&](int rows_per_cta, int ctas_per_sm) {
-        const int need = (rows + rows_per_cta - 1) / rows_per_cta, most = sms * std::min(ctas_per_sm, norm_bwd_ctas(H));
+        const int ctas = sms * std::min(ctas_per_sm, norm_bwd_ctas(H));
+        const int need = (rows + rows_per_cta - 1) / rows_per_cta, most = ragged ? ctas / V * V : ctas;
         return parts = need < most ? need : most;
     };
     auto go = [&](auto kernel, int threads, int rows_per_cta, int ctas_per_sm) {
@@ -709,29 +748,34 @@ static int launch_norm_bwd(const void* dy, const void* dr, const void* r, const 
                             static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r), rstd,
                             static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial, shape.ring);
     };
-    int done_rc = DK_OK;
-    switch (plan) {
-        case NormPlan::VEC_FEW: done_rc = go(add_rms_norm_bwd_kernel<T, W, V, 1, 1024, FROM_REGS>, round_threads(n, 1), 1, 1); break;
-        case NormPlan::VEC_FEW2: done_rc = go(add_rms_norm_bwd_kernel<T, W, V, 2, 1024, FROM_REGS>, round_threads(n, 2), 1, 1); break;
-        case NormPlan::VEC_MANY: {
-            const auto kernel = add_rms_norm_bwd_kernel<T, W, V, 4, 256, FROM_RING>;
-            static bool allowed[64] = {false};
-            done_rc = allow_smem(kernel, allowed);
-            if (done_rc == DK_OK) done_rc = ring_shape(n, H, sizeof(T), dr != nullptr ? 3 : 2, &shape);
-            if (done_rc == DK_OK) done_rc = go(kernel, shape.threads, 1, shape.ctas);
-            break;
+    auto planned = [&](auto is_ragged) {
+        constexpr bool R = decltype(is_ragged)::value;
+        switch (plan) {
+            case NormPlan::FEW: return go(add_rms_norm_bwd_kernel<T, W, 1, 1024, FROM_REGS, R>, round_threads(n, 1), 1, 1);
+            case NormPlan::FEW2: return go(add_rms_norm_bwd_kernel<T, W, 2, 1024, FROM_REGS, R>, round_threads(n, 2), 1, 1);
+            case NormPlan::MANY: {
+                if constexpr (R) {
+                    return go(add_rms_norm_bwd_kernel<T, W, 4, 256, FROM_REGS, true>, round_threads(n, 4), 1,
+                              256 / round_threads(n, 4));
+                } else {
+                    const auto kernel = add_rms_norm_bwd_kernel<T, W, 4, 256, FROM_RING, false>;
+                    static bool allowed[64] = {false};
+                    int rc2 = allow_smem(kernel, allowed);
+                    if (rc2 == DK_OK) rc2 = ring_shape(n, H, sizeof(T), dr != nullptr ? 3 : 2, &shape);
+                    return rc2 != DK_OK ? rc2 : go(kernel, shape.threads, 1, shape.ctas);
+                }
+            }
+            case NormPlan::MANY512: return go(add_rms_norm_bwd_kernel<T, W, 4, 512, FROM_REGS, R>, round_threads(n, 4), 1, 1);
+            default: return go(add_rms_norm_bwd_kernel<T, W, 4, 256, FROM_WARP, R>, 256, 8, 2);
         }
-        case NormPlan::VEC_MANY512: done_rc = go(add_rms_norm_bwd_kernel<T, W, V, 4, 512, FROM_REGS>, round_threads(n, 4), 1, 1); break;
-        case NormPlan::VEC_WARP: done_rc = go(add_rms_norm_bwd_kernel<T, W, V, 4, 256, FROM_WARP>, 256, 8, 2); break;
-        case NormPlan::ONE_FEW: done_rc = go(add_rms_norm_bwd_kernel<T, W, 1, 8, 1024, FROM_REGS>, round_threads(n, 8), 1, 1); break;
-        case NormPlan::ONE_MANY: done_rc = go(add_rms_norm_bwd_kernel<T, W, 1, 16, 512, FROM_REGS>, round_threads(n, 16), 1, 2); break;
-        case NormPlan::ONE_WARP: done_rc = go(add_rms_norm_bwd_kernel<T, W, 1, 8, 256, FROM_WARP>, 256, 8, 2); break;
-        case NormPlan::WIDE:
-            done_rc = launch_early(add_rms_norm_bwd_wide_kernel<T, W>, dim3(grid(1, 2)), NORM_THREADS, 0, 0, st,
-                                   static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r), rstd,
-                                   static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial);
-            break;
-    }
+    };
+    int done_rc;
+    if (plan == NormPlan::WIDE)
+        done_rc = launch_early(add_rms_norm_bwd_wide_kernel<T, W>, dim3(grid(1, 2)), NORM_THREADS, 0, 0, st,
+                               static_cast<const T*>(dy), static_cast<const T*>(dr), static_cast<const T*>(r), rstd,
+                               static_cast<const W*>(weight), rows, H, static_cast<T*>(dx), partial);
+    else
+        done_rc = ragged ? planned(std::true_type{}) : planned(std::false_type{});
     if (done_rc != DK_OK) return done_rc;
     return launch_early(add_rms_norm_dw_kernel<W>, dim3((H + 31) / 32), 256, 0, 0, st, static_cast<const float*>(partial), parts, H,
                         static_cast<W*>(dw));

@@ -17,7 +17,9 @@ DT = {"bf16": torch.bfloat16, "f32": torch.float32}
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
 # rows x width: single rows, widths below a vector, odd, prime, wide; more rows than CTAs
 SHAPES = [(1, 1), (1, 8192), (2, 7), (3, 8), (5, 33), (7, 250), (129, 1000), (64, 5003), (33, 4096), (3, 16384), (2, 65536),
-          (1000, 136), (4099, 64), (700, 2560)]
+          (1000, 136), (4099, 64), (700, 2560),
+          # rows that start on no 16-byte boundary, in every plan: a CTA for a few rows, many, a warp to a row, 512 threads
+          (1000, 137), (4099, 65), (700, 2561), (146, 1003), (148, 2050), (149, 6001), (300, 9001), (3, 10001), (1300, 1), (600, 15)]
 
 
 def make(T, H, dtype, wdtype, residual, seed=0):
