@@ -374,8 +374,8 @@ add_rms_norm_kernel(const T* x, const T* residual, const W* weight, int rows, in
     }
 }
 
-// Any width and alignment: a pass that adds, keeps r and sums the squares, and a pass that writes y. A thread
-// meets the same elements in both, so r_out may be the residual's or x's own buffer.
+// Rows of more than 2048 vectors, and tensors that do not start on 16 bytes: a pass that adds, keeps r and sums the squares,
+// and a pass that writes y. A thread meets the same elements in both, so r_out may be the residual's or x's own buffer.
 template <typename T, typename W, bool MX>
 __global__ void __launch_bounds__(NORM_THREADS)
 add_rms_norm_wide_kernel(const T* x, const T* residual, const W* weight, int rows, int H, float eps, T* r_out,
@@ -556,7 +556,7 @@ add_rms_norm_bwd_kernel(const T* dy, const T* dr, const T* r,
     }
 }
 
-// Any width and alignment.
+// The same rows, backward.
 template <typename T, typename W>
 __global__ void __launch_bounds__(NORM_THREADS)
 add_rms_norm_bwd_wide_kernel(const T* dy, const T* dr, const T* r,
@@ -617,6 +617,7 @@ add_rms_norm_dw_kernel(const float* partial, int parts, int H, W* __restrict__ d
 // host side
 
 constexpr int NORM_MAX_H = 65536;
+constexpr int NORM_MAX_T = 1 << 30;  // a row index plus the rows of a turn stays an int
 constexpr int NORM_MAX_SMS = 160;
 // CTAs of a backward pass on one SM at most, each with a row of `partial`: two, and for narrow rows as many as have
 // 32 KB of partial sums between them
@@ -624,7 +625,7 @@ static int norm_bwd_ctas(int H) { return std::max(2, std::min(8, 8192 / H)); }
 static int norm_bwd_parts(int T, int H) { return std::min(T, NORM_MAX_SMS * norm_bwd_ctas(H)); }
 
 static int check_norm(const void* x, const void* weight, int x_is_f32, int w_is_f32, int T, int H) {
-    DK_REQUIRE(T >= 0, "the number of rows must not be negative");
+    DK_REQUIRE(T >= 0 && T <= NORM_MAX_T, "the number of rows must be between 0 and 2^30");
     DK_REQUIRE(H >= 1 && H <= NORM_MAX_H, "H must be between 1 and 65536");
     DK_REQUIRE(weight != nullptr && (T == 0 || x != nullptr), "null operand");
     DK_REQUIRE(w_is_f32 || !x_is_f32, "a bf16 weight needs bf16 rows");
@@ -820,7 +821,7 @@ extern "C" int dk_add_rms_norm_mx(const void* x, const void* residual, const voi
 
 extern "C" size_t dk_add_rms_norm_bwd_workspace_bytes(int T, int H) {
     using namespace dk;
-    if (T < 0 || H < 1 || H > NORM_MAX_H) return 0;
+    if (T < 0 || T > NORM_MAX_T || H < 1 || H > NORM_MAX_H) return 0;
     return static_cast<size_t>(norm_bwd_parts(T, H)) * H * sizeof(float);
 }
 

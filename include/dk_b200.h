@@ -486,8 +486,8 @@ int dk_moe_ep_layer(const dk_moe_ep_args* args, const dk_view* view, unsigned ep
 /* ------------------------------------------------------------------ norm with the residual's addition */
 /*
  * No counterpart in the reference's distributed path. Rows of H values, bf16 or (x_is_f32 != 0) fp32;
- * the weight has the type of the rows or (w_is_f32 != 0) fp32. 1 <= H <= 65536, any T >= 0 (T == 0
- * launches nothing). All sums in fp32.
+ * the weight has the type of the rows or (w_is_f32 != 0) fp32. 1 <= H <= 65536, 0 <= T <= 2^30 (T == 0
+ * launches nothing). All sums in fp32. Rows are fastest up to 2048 16-byte vectors, in tensors that start on 16 bytes.
  *   r = x + residual, rounded to the type of the rows (residual == NULL: r = x, and r_out is NULL too)
  *   y = r * rstd * weight, rstd = 1 / sqrt(mean(r^2) + eps)
  * r_out may be the buffer of residual or of x (the stream updated in place); any other overlap of an
@@ -502,6 +502,10 @@ int dk_moe_ep_layer(const dk_moe_ep_args* args, const dk_view* view, unsigned ep
  * dx [T, H] (the gradient of x and of residual) and dw [H] in the type of the weight. workspace:
  * dk_add_rms_norm_bwd_workspace_bytes(T, H) bytes, 16-byte aligned, contents undefined before and after.
  * The same inputs give the same bits on every run on one model of GPU.
+ *
+ * These calls and dk_gated_ffn* may be captured into a CUDA graph after one eager call of each on the device (what they set up
+ * lazily is set up there). Their kernels may set themselves up while the kernel before them on the stream still runs
+ * (programmatic stream serialization) but read and write in stream order. Calls on different streams are independent.
  */
 int dk_add_rms_norm(const void* x, const void* residual, const void* weight, int x_is_f32, int w_is_f32, int T, int H,
                     float eps, void* y, void* r_out, float* rstd, void* stream);

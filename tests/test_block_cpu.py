@@ -45,7 +45,7 @@ def test_c_abi_argument_errors(capi):
     L, one = capi.lib(), _p(4096)
     norm = lambda T=4, H=64, x=one, w=one, xf=0, wf=0, eps=1e-6, y=one, res=None, r=None: L.dk_add_rms_norm(
         x, res, w, xf, wf, T, H, eps, y, r, one, None)
-    bad = [norm(T=-1), norm(H=0), norm(H=65537), norm(x=None), norm(w=None), norm(y=None), norm(xf=1, wf=0), norm(eps=0.0),
+    bad = [norm(T=-1), norm(T=(1 << 30) + 1), norm(H=0), norm(H=65537), norm(x=None), norm(w=None), norm(y=None), norm(xf=1, wf=0), norm(eps=0.0),
            norm(eps=-1.0), norm(eps=float("nan")), norm(eps=float("inf")), norm(res=one), norm(r=one), norm(x=_p(4097)), norm(y=_p(4097)), norm(w=_p(4097)), norm(x=_p(4098), xf=1, wf=1)]
     assert bad == [capi.ERR_ARG] * len(bad)
     assert norm(T=0, x=None, y=None) == 0
