@@ -422,6 +422,33 @@ def test_the_block_as_it_is_trained(ops, orc):
         assert orc.rel_fro(a.grad.double().cpu(), b.grad.cpu()) <= 4 * R
 
 
+def test_captured_gradients(ops):
+    """A step through autograd captured when no eager graph of its leaves is alive, and explicit calls captured while one is."""
+    leaves = [t.cuda().requires_grad_() for t in make(40, 64, 128)[:3]]
+    dy = make(40, 64, 128)[3].cuda()
+    y = ops.gated_ffn_train(*leaves)[0]
+    y.backward(dy)
+    want = [t.grad.clone() for t in leaves]
+    del y
+    for t in leaves:
+        t.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.gated_ffn_train(*leaves)[0].backward(dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+    alive = ops.gated_ffn_train(*leaves)[0]
+    plain = [t.detach() for t in leaves]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, gu, h = ops.gated_ffn_train(*plain)
+        got = ops.gated_ffn_bwd(dy, *plain, gu, h)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and alive.grad_fn is not None
+
+
 def test_autograd_alone(ops, orc):
     """rms_norm and gated_ffn_train with an expanded incoming gradient, and an output nobody uses."""
     x, w13, w2, dy = (t.cuda() for t in make(20, 64, 128))
