@@ -902,6 +902,17 @@ static int products(const Spec* s, int count, void* gu, cudaStream_t st) {
     return t.pair == 2 ? launch<EPI, 2>(maps, g, st) : launch<EPI, 1>(maps, g, st);
 }
 
+// Tokens of a tile: all of them (up to 256), or near 64, above 256 rows near 96, where the weights come from L2 when they
+// are read again, and the shorter epilogue and the larger number of CTAs are worth more (training steps: 140 rows of
+// 2048 x 4096 71 us against 80, 256 rows 81 against 95; of 4096 x 4096, 64 MB, 119 against 103). Tiles are equally full.
+constexpr size_t SMALL_WEIGHTS = 32u << 20;
+static int rows_tokens(int T, size_t weights) {
+    int most = 256;
+    if (weights <= SMALL_WEIGHTS) most = T <= 256 || weights <= SMALL_WEIGHTS / 2 ? 64 : 96;
+    const int tiles = (T + most - 1) / most;
+    return ((T + tiles - 1) / tiles + 15) / 16 * 16;
+}
+
 // out [T, cols] = x W^T for few rows. GATED: W = W13, out = h; DGATED: x = dy, out = dgu. W_MN: W is [K, cols].
 template <int EPI, bool W_MN>
 static int rows_product(const void* x, const void* W, void* out, int T, int cols, int K, void* gu, bool follows,
@@ -913,11 +924,7 @@ static int rows_product(const void* x, const void* W, void* out, int T, int cols
     if (rc == DK_OK) rc = sm_count(&sms);
     if (rc != DK_OK) return rc;
     const bool gated = EPI == EPI_GATED;
-    // Tokens of a tile: all of them, or 64 where reading the weights again is cheap (up to 16 MB they come from L2) and the
-    // shorter epilogue and the larger number of CTAs are worth more (256 rows of 1536 x 2048: 21.4 us against 26.6;
-    // of 8192 x 3584: 80 against 66).
-    const size_t weights = static_cast<size_t>(gated ? 2 : 1) * cols * K * 2;
-    const int N = T > 64 && weights <= (16u << 20) ? 64 : std::min(256, (T + 15) / 16 * 16);
+    const int N = rows_tokens(T, static_cast<size_t>(gated ? 2 : 1) * cols * K * 2);
     RowsMaps maps;
     rc = operand_map(&maps.w, W, W_MN, gated ? 2 * cols : cols, K, gated ? 64 : 128);
     if (rc == DK_OK) rc = operand_map(&maps.x, x, false, T, K, N);
@@ -941,8 +948,14 @@ static int rows_product(const void* x, const void* W, void* out, int T, int cols
     return launch_early(kernel, dim3(tiles * S, token_tiles), ROWS_THREADS, rows_smem(N), S, st, maps, g);
 }
 
-// Few rows: see ffn_rows_kernel.
-constexpr int ROWS_MAX_T = 256;
+// Whether a call's products go by ffn_rows_kernel: up to 256 rows, and more where the weights are small. Measured, training
+// steps, against ffn_gemm_kernel: 300 rows of 1536 x 2048 (12 MB) 53 us against 71, 513 62 against 77, 700 77 against 80 (forward
+// alone 32 against 26); 300 rows of 2048 x 4096 (32 MB) 89 against 123, 384 99 against 121, 513 136 against 141 (forward 49
+// against 45); 384 rows of 4096 x 4096 (64 MB) 178 against 174.
+static bool few_rows(int T, int H, int F) {
+    const size_t w13 = static_cast<size_t>(4) * F * H;
+    return T <= (w13 <= SMALL_WEIGHTS / 2 ? 576 : w13 <= SMALL_WEIGHTS ? 400 : 256);
+}
 
 static int check_shape(int T, int H, int F) {
     DK_REQUIRE(T >= 0, "the number of rows must not be negative");
@@ -973,7 +986,7 @@ extern "C" int dk_gated_ffn(const void* x, const void* w13, const void* w2, int 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     rc = check_aligned({x, w13, w2, gu, h, y});
     if (rc != DK_OK) return rc;
-    if (T <= ROWS_MAX_T) {
+    if (few_rows(T, H, F)) {
         rc = rows_product<EPI_GATED, false>(x, w13, h, T, F, H, gu, false, st);
         if (rc != DK_OK) return rc;
         return rows_product<EPI_STORE, false>(h, w2, y, T, H, F, nullptr, true, st);
@@ -1002,7 +1015,7 @@ extern "C" int dk_gated_ffn_bwd(const void* dy, const void* x, const void* w13, 
     if (rc != DK_OK) return rc;
     // dW13 [2F,H] = dgu^T x and dW2 [H,F] = dy^T h, the tokens as K
     const Spec d_w13{dgu, x, dw13, 2 * F, H, T, true, true}, d_w2{dy, h, dw2, H, F, T, true, true};
-    if (T <= ROWS_MAX_T) {
+    if (few_rows(T, H, F)) {
         // dh = dy W2 straight into dg and du, then dx = dgu W13
         rc = rows_product<EPI_DGATED, true>(dy, w2, dgu, T, F, H, const_cast<void*>(gu), false, st);
         if (rc == DK_OK) rc = rows_product<EPI_STORE, true>(dgu, w13, dx, T, H, 2 * F, nullptr, true, st);
