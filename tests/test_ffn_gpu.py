@@ -70,7 +70,9 @@ def bounds(x, w13, w2, dy):
 SHAPES = [(1, 512, 256), (2, 64, 64), (3, 8, 8), (5, 256, 72), (16, 1032, 136), (17, 520, 1000), (31, 2048, 4096), (33, 72, 2056),
           (64, 4096, 512), (65, 128, 128), (100, 512, 768), (127, 136, 264), (128, 256, 256), (129, 384, 640), (200, 1024, 136),
           (255, 264, 392), (257, 320, 1288), (513, 512, 520), (700, 2056, 1032),
-          (1000, 4104, 1544), (1357, 2048, 3592), (600, 3592, 5128), (2100, 2056, 2568)]
+          (1000, 4104, 1544), (1357, 2048, 3592), (600, 3592, 5128), (2100, 2056, 2568),
+          # large weights: token tiles of more than 128, and the tile kernel from 257 rows on
+          (150, 4104, 2056), (256, 2056, 4104), (260, 4104, 2056)]
 
 
 @pytest.mark.parametrize("T,H,F", SHAPES)
@@ -110,7 +112,7 @@ def test_every_element_of_every_tile(orc):
     """Weights that route single inputs to single outputs: each value of y is one value of x, exactly, so a tile that
     is swapped, shifted or dropped shows. g = 32 (sigmoid(32) is 1 in fp32), u = x, h = 32 x, y = 32 x / 32."""
     import tk_kernel as tk
-    for T, H in ((1, 512), (130, 640), (300, 264)):
+    for T, H in ((1, 512), (130, 640), (300, 264), (700, 264)):
         F = H - 8
         x = torch.randint(-64, 64, (T, H), generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
         x[:, -1] = 1
@@ -148,7 +150,7 @@ def test_extreme_gates():
 
 def test_non_finite_rows_stay_in_their_rows(orc):
     import tk_kernel as tk
-    for T in (6, 300):
+    for T in (6, 300, 700):
         x, w13, w2, _ = make(T, 256, 136)
         good = tk.gated_ffn(x.cuda(), w13.cuda(), w2.cuda())
         x[2, 5] = float("nan")
@@ -161,7 +163,7 @@ def test_non_finite_rows_stay_in_their_rows(orc):
 def test_rows_do_not_depend_on_their_batch_neighbours(orc):
     """A row's result depends on that row and its place alone."""
     import tk_kernel as tk
-    for T, H, F in ((7, 512, 264), (150, 512, 264), (400, 512, 264), (1357, 2048, 1032)):
+    for T, H, F in ((7, 512, 264), (150, 512, 264), (400, 512, 264), (700, 512, 264), (1357, 2048, 1032)):
         x, w13, w2, _ = make(T, H, F)
         other = make(T, H, F, seed=1)[0]
         keep = torch.arange(0, T, 3)
@@ -240,7 +242,7 @@ def test_operators_pass_opcheck(ops):
         torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
 
 
-@pytest.mark.parametrize("T", [4, 260])
+@pytest.mark.parametrize("T", [4, 260, 700])
 def test_two_streams_at_once_and_graph(T):
     """Two calls that overlap on the GPU, and a captured step replayed on other inputs."""
     import tk_kernel as tk
@@ -280,7 +282,7 @@ def test_two_streams_at_once_and_graph(T):
             assert all(torch.equal(u, v) for u, v in zip(out, w))
 
 
-@pytest.mark.parametrize("T", [3, 260])
+@pytest.mark.parametrize("T", [3, 260, 700])
 def test_order_with_other_work(T):
     """The calls may set themselves up while earlier work runs, but read and write in order: after copies, memsets, torch's
     kernels and events of another stream, before torch's kernels, over buffers that are used again and again, eager and
