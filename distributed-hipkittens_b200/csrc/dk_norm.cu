@@ -587,6 +587,99 @@ add_rms_norm_bwd_wide_kernel(const T* dy, const T* dr, const T* r,
     }
 }
 
+// Few rows, backward in one launch: dw needs the rows' rstd but not their sums, so the first `rows` CTAs make dx, a row each, and
+// the others dw, 64 columns each, reading dy and r once more (from L2). A step of 7 rows of 4176 with its forward pass
+// takes 18.6 us instead of 22.4, which are the host's: a launch and a buffer less. WIDE: rows that do not fit into
+// registers, and tensors that do not start on 16 bytes.
+template <typename T, typename W, int VPT, bool RAGGED, bool WIDE>
+__global__ void __launch_bounds__(1024)
+add_rms_norm_bwd_few_kernel(const T* dy, const T* dr, const T* r, const float* rstd_in, const W* weight, int rows, int H, T* dx,
+                            W* dw) {
+    constexpr int V = 16 / sizeof(T);
+    __shared__ float part[2][32];
+    __shared__ float sum[32][64];
+    next_may_begin();
+    previous_done();
+    const int tid = threadIdx.x, threads = blockDim.x;
+    if (static_cast<int>(blockIdx.x) < rows) {
+        const int row = blockIdx.x;
+        const size_t base = static_cast<size_t>(row) * H;
+        const float rstd = rstd_in[row];
+        if constexpr (WIDE) {
+            float dot = 0.f;
+            for (int c = tid; c < H; c += threads) dot += to_f32(dy[base + c]) * to_f32(weight[c]) * (to_f32(r[base + c]) * rstd);
+            const float mean = row_sum<false>(dot, part, 0, threads) / static_cast<float>(H);
+            for (int c = tid; c < H; c += threads) {
+                const float n = to_f32(r[base + c]) * rstd;
+                float v = rstd * (to_f32(dy[base + c]) * to_f32(weight[c]) - n * mean);
+                if (dr != nullptr) v += to_f32(dr[base + c]);
+                dx[base + c] = from_f32<T>(v);
+            }
+        } else {
+            const RowVectors<V, RAGGED> at(row, H);
+            Pack<T, V> d[VPT], h[VPT], above[VPT];
+            Pack<W, V> w[VPT];
+            float dot = 0.f;
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int i = j * threads + tid;
+                d[j].zero();
+                h[j].zero();
+                above[j].zero();
+                w[j].zero();
+                if (i < at.count) {
+                    at.load(d[j], dy + base, i);
+                    at.load(h[j], r + base, i);
+                    if (dr != nullptr) at.load(above[j], dr + base, i);
+                    at.load_weight(w[j], weight, i);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < VPT; ++j)
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    dot += to_f32(d[j].e[k]) * (to_f32(h[j].e[k]) * rstd) * to_f32(w[j].e[k]);
+            const float mean = row_sum<false>(dot, part, 0, threads) / static_cast<float>(H);
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int i = j * threads + tid;
+                if (i < at.count) {
+                    Pack<T, V> o;
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        const float n = to_f32(h[j].e[k]) * rstd;
+                        float v = rstd * (to_f32(d[j].e[k]) * to_f32(w[j].e[k]) - n * mean);
+                        if (dr != nullptr) v += to_f32(above[j].e[k]);
+                        o.e[k] = from_f32<T>(v);
+                    }
+                    at.store(o, dx + base, i);
+                }
+            }
+        }
+        return;
+    }
+    // warp w adds up rows w, w + warps, ...; the warps' sums are added up in order
+    const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+    const int c0 = (blockIdx.x - rows) * 64 + lane, c1 = c0 + 32;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
+    for (int row = warp; row < rows; row += warps) {
+        const size_t base = static_cast<size_t>(row) * H;
+        const float rstd = rstd_in[row];
+        if (c0 < H) s0 += to_f32(dy[base + c0]) * (to_f32(r[base + c0]) * rstd);
+        if (c1 < H) s1 += to_f32(dy[base + c1]) * (to_f32(r[base + c1]) * rstd);
+    }
+    sum[warp][lane] = s0;
+    sum[warp][lane + 32] = s1;
+    __syncthreads();
+    const int c = (blockIdx.x - rows) * 64 + tid;
+    if (tid < 64 && c < H) {
+        float v = 0.f;
+        for (int q = 0; q < warps; ++q) v += sum[q][tid];
+        dw[c] = from_f32<W>(v);
+    }
+}
+
 // dw[c] = sum of the CTAs' partial sums: 32 columns to a CTA, its eight warps each take every eighth part, and
 // their sums are added up in order. Launched while the backward pass still runs (its CTAs fit beside that one's), it
 // waits for its end on the device.
@@ -622,7 +715,11 @@ constexpr int NORM_MAX_SMS = 160;
 // CTAs of a backward pass on one SM at most, each with a row of `partial`: two, and for narrow rows as many as have
 // 32 KB of partial sums between them
 static int norm_bwd_ctas(int H) { return std::max(2, std::min(8, 8192 / H)); }
-static int norm_bwd_parts(int T, int H) { return std::min(T, NORM_MAX_SMS * norm_bwd_ctas(H)); }
+// Up to so many rows a backward pass is one launch without partial sums. In device time, bf16: 128 rows of 8192 5.4 us
+// instead of 7.8 + 7.5 in two overlapping launches, of 4176 4.6 instead of 5.0 + 5.0; 512 rows of 4176 12.7 instead of
+// 8.7 + 8.3: a column's rows are added up by one CTA here.
+constexpr int NORM_BWD_FEW = 128;
+static int norm_bwd_parts(int T, int H) { return T <= NORM_BWD_FEW ? 0 : std::min(T, NORM_MAX_SMS * norm_bwd_ctas(H)); }
 
 static int check_norm(const void* x, const void* weight, int x_is_f32, int w_is_f32, int T, int H) {
     DK_REQUIRE(T >= 0 && T <= NORM_MAX_T, "the number of rows must be between 0 and 2^30");
@@ -643,14 +740,14 @@ static int check_elements(int x_is_f32, int w_is_f32, std::initializer_list<cons
 }
 
 // How a pass over T rows of H elements is cut up. n: vectors a row may span.
-//   FEW      at most one row for each SM: as many threads to a row as it can use (latency)
+//   FEW      at most `few` rows, no more than a row for each SM: as many threads to a row as it can use (latency)
 //   MANY     four vectors a thread, so that a CTA has enough bytes in flight (bandwidth)
 //   WARP     rows of at most 4 vectors a lane: a row to a warp, no barrier
 //   WIDE     a row that does not fit into the registers of 512 threads, or tensors that do not start on 16 bytes
 enum class NormPlan { FEW, FEW2, MANY, MANY512, WARP, WIDE };
-static NormPlan norm_plan(bool aligned, int n, int T, int sms) {
+static NormPlan norm_plan(bool aligned, int n, int T, int few) {
     if (!aligned || n > 2048) return NormPlan::WIDE;
-    if (T <= sms) return n <= 1024 ? NormPlan::FEW : NormPlan::FEW2;
+    if (T <= few) return n <= 1024 ? NormPlan::FEW : NormPlan::FEW2;
     if (n <= 128) return NormPlan::WARP;
     return n <= 1024 ? NormPlan::MANY : NormPlan::MANY512;
 }
@@ -736,7 +833,21 @@ static int launch_norm_bwd(const void* dy, const void* dr, const void* r, const 
     if (sms > NORM_MAX_SMS) sms = NORM_MAX_SMS;
     const bool ragged = H % V != 0;
     const int n = ragged ? (H + 2 * V - 2) / V : H / V;
-    const NormPlan plan = norm_plan(aligned16({dy, dr, r, weight, dx}), n, rows, sms);
+    const NormPlan plan = norm_plan(aligned16({dy, dr, r, weight, dx}), n, rows, NORM_BWD_FEW);
+    if (rows <= NORM_BWD_FEW) {
+        auto few = [&](auto kernel, int threads) {
+            // 512 threads at least, for the CTAs that make dw
+            return launch_early(kernel, dim3(rows + (H + 63) / 64), std::max(512, threads), 0, 0, st, static_cast<const T*>(dy),
+                                static_cast<const T*>(dr), static_cast<const T*>(r), rstd, static_cast<const W*>(weight), rows, H,
+                                static_cast<T*>(dx), static_cast<W*>(dw));
+        };
+        if (plan == NormPlan::WIDE) return few(add_rms_norm_bwd_few_kernel<T, W, 1, false, true>, 1024);
+        if (n <= 1024)
+            return ragged ? few(add_rms_norm_bwd_few_kernel<T, W, 1, true, false>, round_threads(n, 1))
+                          : few(add_rms_norm_bwd_few_kernel<T, W, 1, false, false>, round_threads(n, 1));
+        return ragged ? few(add_rms_norm_bwd_few_kernel<T, W, 2, true, false>, round_threads(n, 2))
+                      : few(add_rms_norm_bwd_few_kernel<T, W, 2, false, false>, round_threads(n, 2));
+    }
     int parts = 0;
     RingShape shape{};
     auto grid = [&](int rows_per_cta, int ctas_per_sm) {
@@ -752,8 +863,6 @@ static int launch_norm_bwd(const void* dy, const void* dr, const void* r, const 
     auto planned = [&](auto is_ragged) {
         constexpr bool R = decltype(is_ragged)::value;
         switch (plan) {
-            case NormPlan::FEW: return go(add_rms_norm_bwd_kernel<T, W, 1, 1024, FROM_REGS, R>, round_threads(n, 1), 1, 1);
-            case NormPlan::FEW2: return go(add_rms_norm_bwd_kernel<T, W, 2, 1024, FROM_REGS, R>, round_threads(n, 2), 1, 1);
             case NormPlan::MANY: {
                 if constexpr (R) {
                     return go(add_rms_norm_bwd_kernel<T, W, 4, 256, FROM_REGS, true>, round_threads(n, 4), 1,
@@ -839,7 +948,8 @@ extern "C" int dk_add_rms_norm_bwd(const void* dy, const void* dr, const void* r
     }
     DK_REQUIRE(dy != nullptr && rstd != nullptr, "null operand");
     DK_REQUIRE(dx != nullptr, "null output");
-    DK_REQUIRE(workspace != nullptr && workspace_bytes >= dk_add_rms_norm_bwd_workspace_bytes(T, H), "workspace too small");
+    const size_t need = dk_add_rms_norm_bwd_workspace_bytes(T, H);
+    DK_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small");
     DK_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "the workspace must be 16-byte aligned");
     const int rc2 = check_elements(x_is_f32, w_is_f32, {dy, dr, r, dx}, weight, {rstd});
     if (rc2 != DK_OK) return rc2;

@@ -597,10 +597,11 @@ py::tuple add_rms_norm_bwd(py::object dY, py::object dR, py::object R, py::objec
     if (!rs.is(a.T)) throw std::runtime_error("rstd must be [T]");
     want_dtype(rs, t.f32, "rstd", "torch.float32");
     const size_t wb = dk_add_rms_norm_bwd_workspace_bytes(a.T, a.H);
-    void *dxp, *dwp, *wsp;
+    void *dxp, *dwp, *wsp = nullptr;
     py::object dx = empty_like(R, &dxp);
     py::object dw = empty_like(Weight, &dwp);
-    py::object ws = new_empty(R, static_cast<int64_t>(wb / 4), t.f32, &wsp);
+    py::object ws;
+    if (wb > 0) ws = new_empty(R, static_cast<int64_t>(wb / 4), t.f32, &wsp);
     throw_on(dk_add_rms_norm_bwd(dy.ptr, a.res.ptr, a.x.ptr, static_cast<const float*>(rs.ptr), a.w.ptr, a.x_f32, a.w_f32,
                                  a.T, a.H, dxp, dwp, wsp, wb, stream_of(a.device)), "add_rms_norm_bwd");
     return py::make_tuple(dx, dw);

@@ -500,7 +500,8 @@ int dk_moe_ep_layer(const dk_moe_ep_args* args, const dk_view* view, unsigned ep
  * q, s_rows and sf_atoms start on 16 bytes.
  * dk_add_rms_norm_bwd: from dy, r, rstd and (may be NULL) dr, the gradient of r from the layers above:
  * dx [T, H] (the gradient of x and of residual) and dw [H] in the type of the weight. workspace:
- * dk_add_rms_norm_bwd_workspace_bytes(T, H) bytes, 16-byte aligned, contents undefined before and after.
+ * dk_add_rms_norm_bwd_workspace_bytes(T, H) bytes (none up to 128 rows), 16-byte aligned, contents undefined before and
+ * after.
  * The same inputs give the same bits on every run on one model of GPU.
  *
  * These calls and dk_gated_ffn* may be captured into a CUDA graph after one eager call of each on the device (what they set up

@@ -54,10 +54,10 @@ def test_c_abi_argument_errors(capi):
     bad = [mx(H=64), mx(H=192), mx(q=None), mx(s=None), mx(a=None), mx(res=one), mx(q=_p(4100)), mx(a=_p(4104)), mx(s=_p(4097))]
     assert bad == [capi.ERR_ARG] * len(bad)
     assert mx(T=0, q=None) == 0
-    wb = L.dk_add_rms_norm_bwd_workspace_bytes(4, 64)
-    assert wb >= 64 * 4 and L.dk_add_rms_norm_bwd_workspace_bytes(-1, 64) == 0 and L.dk_add_rms_norm_bwd_workspace_bytes(4, 0) == 0
+    wb = L.dk_add_rms_norm_bwd_workspace_bytes(200, 64)
+    assert wb >= 64 * 4 and L.dk_add_rms_norm_bwd_workspace_bytes(128, 64) == 0 and L.dk_add_rms_norm_bwd_workspace_bytes(-1, 64) == 0 and L.dk_add_rms_norm_bwd_workspace_bytes(4, 0) == 0
     bwd = lambda dy=one, r=one, rstd=one, w=one, dx=one, dw=one, ws=one, n=wb: L.dk_add_rms_norm_bwd(
-        dy, None, r, rstd, w, 0, 0, 4, 64, dx, dw, ws, n, None)
+        dy, None, r, rstd, w, 0, 0, 200, 64, dx, dw, ws, n, None)
     bad = [bwd(dy=None), bwd(r=None), bwd(rstd=None), bwd(w=None), bwd(dx=None), bwd(dw=None), bwd(ws=None), bwd(n=wb - 1),
            bwd(ws=_p(4100)), bwd(dy=_p(4097)), bwd(dx=_p(4097)), bwd(rstd=_p(4098)), bwd(dw=_p(4097))]
     assert bad == [capi.ERR_ARG] * len(bad)

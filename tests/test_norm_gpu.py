@@ -229,6 +229,29 @@ def test_unaligned_rows_mx(orc):
     check_mx(q, s, atoms, y64, orc)
 
 
+@pytest.mark.parametrize("T", [1, 127, 128, 129])
+@pytest.mark.parametrize("H,dtype", [(63, torch.float32), (65, torch.bfloat16), (512, torch.bfloat16), (5003, torch.float32),
+                                     (8200, torch.bfloat16), (20000, torch.bfloat16)])
+def test_few_rows_backward(orc, capi, T, H, dtype):
+    """Both sides of the one-launch backward pass; guard words around its outputs, called through the C ABI."""
+    x, res, w = make(T, H, dtype, torch.float32, True)
+    dy = torch.randn(T, H, generator=torch.Generator().manual_seed(T + H)).to(dtype)
+    rstd = 1 / (x.double().square().mean(1) + 1e-6).sqrt()
+    rstd = rstd.float()
+    bits, L = dtype.itemsize, capi.lib()
+    wb = L.dk_add_rms_norm_bwd_workspace_bytes(T, H)
+    assert (wb == 0) == (T <= 128)
+    out = {k: torch.full((n + 512,), 0xA5, dtype=torch.uint8, device="cuda") for k, n in (("dx", T * H * bits), ("dw", 4 * H), ("ws", wb))}
+    D, DR, R, S, W = dy.cuda(), res.cuda(), x.cuda(), rstd.cuda(), w.cuda()
+    at = {k: b.data_ptr() + 256 for k, b in out.items()}
+    capi.check(L.dk_add_rms_norm_bwd(D.data_ptr(), DR.data_ptr(), R.data_ptr(), S.data_ptr(), W.data_ptr(), int(bits == 4), 1, T, H,
+                                     at["dx"], at["dw"], at["ws"] if wb else None, wb, capi._stream_ptr(None)))
+    torch.cuda.synchronize()
+    for k, b in out.items():
+        assert (b[:256] == 0xA5).all() and (b[-256:] == 0xA5).all(), k
+    check_bwd(out["dx"][256:-256].view(dtype).view(T, H), out["dw"][256:-256].view(torch.float32), dy, res, x, rstd, w, orc)
+
+
 def test_nothing_is_written_outside(capi):
     """Guard words around every output, called through the C ABI."""
     T, H = 131, 384
