@@ -23,15 +23,17 @@
 // matrix products.
 //
 //   warp 0      TMA producer: 128-byte-swizzled boxes into a ring of stages
-//   warp 1      one thread issues tcgen05.mma into one of two 256-column accumulators
+//   warp 1      an elected thread issues tcgen05.mma into one of two 256-column accumulators
 //   warps 2-5   epilogue: tcgen05.ld, swizzled staging in shared memory, TMA stores (which clip the
 //               ragged edges)
 //
 // PAIR = 2: a cluster of two CTAs per 256x256 tile (cta_group::2). Each stages its 128 rows of A and half of
 // the B tile (gated: CTA 0 the gate rows, CTA 1 the up rows), so a stage is 32 KiB instead of 48, the ring six
 // deep instead of four, and a flop needs two thirds of the shared-memory fill. Both CTAs' loads complete on the
-// leader's barrier, the leader issues the MMAs. PAIR = 1: one CTA per 128x256 tile, for row counts whose last pair
-// would be half empty.
+// leader's barrier, the leader issues the MMAs. PAIR = 1: one CTA per tile of 128 rows, where pairs would leave
+// rows or a last wave half empty (choose()).
+//
+// Few rows go by a kernel of their own with the weights as A, ffn_rows_kernel below; few_rows() says when.
 #include "dk_host.h"
 #include "dk_launch.cuh"
 #include "dk_ptx.cuh"
@@ -809,7 +811,7 @@ struct Spec {
 // (in units of a pair's 256 columns, 0.335 us), and its epilogue, overlapped with the next tile's K blocks:
 //   two CTAs    256 columns 1.0   192 columns 0.85   128 columns 0.8
 //   one CTA     256 columns 1.1   192 columns 0.95   128 columns 0.75
-// Wide pairs are fastest per flop (they load least per flop; 128 columns are bound by L2); narrow tiles and single CTAs cut
+// Wide pairs are fastest per flop (they load least per flop; 128 columns are bound by shared-memory bandwidth); narrow tiles and single CTAs cut
 // the work finer where it would not go evenly into waves, or compute fewer rows for nothing. 192 columns only where
 // nothing but a K-major B is loaded and stored.
 struct Tiling {
